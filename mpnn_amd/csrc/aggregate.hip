@@ -34,8 +34,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// edge_term for pairs of columns, as vector arithmetic (v_pk_mul_f32 / v_pk_fma_f32): per column the same multiply
-// and fma chain in f order.
+// edge_term for pairs of columns, as vector arithmetic (one instruction per column: the build leaves the packed float32
+// instructions out): per column the same multiply and fma chain in f order.
 template <int VEC, int FE>
 __device__ __forceinline__ void edge_term_pairs(const float (&w)[VEC][FE], const float (&e)[FE], float (&ce)[VEC]) {
 #pragma unroll
@@ -276,9 +276,8 @@ __global__ void __launch_bounds__(kBlock, fwd_waves(VEC, FE)) k_agg_fwd(FwdArgs<
             else edge_term<VEC, FE>(w, ev, ce);
             RowIO<T, VEC>::unpack(braw[u], bv);
             if constexpr (OWN) {
-              // the pre-activations of column pairs on packed instructions, written as vector arithmetic: their
-              // results go into the block below lane register by lane register, and the compiler does not pair up
-              // scalar arithmetic that feeds it (same operations in the same order as the scalar form)
+              // the pre-activations of column pairs, written as vector arithmetic (same operations in the same order
+              // as the scalar form)
               float m[VEC];
 #pragma unroll
               for (int q = 0; q < VEC / 2; ++q) {

@@ -1152,12 +1152,12 @@ __device__ __forceinline__ RegionBlock region_block(const int32_t* island_ptr, i
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ f32x2 fma2(f32x2 a, float b, f32x2 c) {   // v_pk_fma_f32, b for both halves
+__device__ __forceinline__ f32x2 fma2(f32x2 a, float b, f32x2 c) {   // b for both halves (one fma per half)
   return __builtin_elementwise_fma(a, (f32x2)(b), c);
 }
 
 // The lane's rows of the node weight (A and B halves) and of the edge weight: columns 4 (lane % 16) + 2 p and + 1
-// as pair p, so that a multiply-add serves two columns (v_pk_fma_f32).  FEW: attribute values taken per edge (1,
+// as pair p.  FEW: attribute values taken per edge (1,
 // or 8 with zeros past the real width); FW: values taken per row of x (3 or 4).
 template <typename T, int FEW, int FW>
 struct ThinWeights {
