@@ -40,7 +40,7 @@ enum {
   MPNN_E_CAPACITY = -4   /* an output array's stated capacity is too small */
 };
 
-#define MPNN_ABI_VERSION 17
+#define MPNN_ABI_VERSION 18
 
 /* Library self-description. */
 int32_t mpnn_abi_version(void);
@@ -592,6 +592,39 @@ int32_t mpnn_region_layer_fwd(const mpnn_island_layer* desc, int32_t max_nodes, 
 int32_t mpnn_region_layer_bwd(const mpnn_island_layer* desc, int32_t max_nodes, const int32_t* rowptr_t,
                               const int32_t* col_t, const void* ea_t, const float* aggr, float* ga,
                               mpnn_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Residual join with the norms around it (no counterpart in the reference; it stands between the layers of
+ * models/layers.py:11-140 in a deep stack).  Per row of H columns, in float32:
+ *   n      = post ? norm(block) * post_w + post_b : block
+ *   stream = residual_scale * residual + branch_scale * gate * n
+ *   normed = norm(stream) * w + b
+ * norm(v) = v / sqrt(mean(v^2) + eps) (MPNN_NORM_RMS) or (v - mean) / sqrt(var(v) + eps) (MPNN_NORM_LAYER).
+ * block, residual [N, H]; gate by gate_kind: none, [H], one value per row ([N] with stride ldg), or [N, H]; post_w,
+ * post_b, w, b [H] or NULL (1 and 0); residual NULL counts as zeros.  All of one dtype; 1 <= H <= 2048.  Rows move
+ * as 16-byte vectors when H, every address and every row stride allow it, column by column otherwise.
+ *
+ * mpnn_block_norm_fwd writes stream and / or normed (a NULL one is not computed).
+ * mpnn_block_norm_bwd reads the forward's inputs again and g_stream, g_normed (NULL: zeros), and writes whichever of
+ *   g_block, g_residual [N, H], g_gate (shaped as gate), g_post_w, g_post_b, g_w, g_b [H] is not NULL.  `partial`:
+ *   mpnn_block_norm_partial_floats(N, H, dtype) floats of scratch.  Sums over rows are added in a fixed order.
+ * ------------------------------------------------------------------------- */
+enum { MPNN_NORM_RMS = 0, MPNN_NORM_LAYER = 1 };
+enum { MPNN_GATE_NONE = 0, MPNN_GATE_CHANNEL = 1, MPNN_GATE_ROW = 2, MPNN_GATE_FULL = 3 };
+typedef struct mpnn_block_norm {
+  const void* block; int64_t ldb; const void* residual; int64_t ldr; const void* gate; int64_t ldg;
+  const void* post_w; const void* post_b; const void* w; const void* b;
+  int64_t N; int32_t H; int32_t dtype; int32_t norm; int32_t gate_kind; int32_t post;
+  float eps; float residual_scale; float branch_scale;
+  void* stream; int64_t lds; void* normed; int64_t ldn;
+  const void* g_stream; int64_t ldgs; const void* g_normed; int64_t ldgn;
+  void* g_block; int64_t ldgb; void* g_residual; int64_t ldgr; void* g_gate; int64_t ldgg;
+  void* g_post_w; void* g_post_b; void* g_w; void* g_b;
+  float* partial;
+} mpnn_block_norm;
+int64_t mpnn_block_norm_partial_floats(int64_t N, int32_t H, int32_t dtype);
+int32_t mpnn_block_norm_fwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
+int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,7 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 MPNN_F32 = 0
 MPNN_BF16 = 1
 MPNN_U8 = 2
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 LIB_PATH = os.environ.get("MPNN_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmpnn_amd.so")
 
@@ -53,6 +53,22 @@ class IslandLayerDesc(ctypes.Structure):
         ("gx", c_void_p), ("ldgx", c_int64), ("gpos", c_void_p),
         ("g_wn", c_void_p), ("g_we", c_void_p), ("g_wout", c_void_p), ("g_wpos", c_void_p),
         ("partial", c_void_p), ("gx_part", c_void_p),
+    ]
+
+
+class BlockNormDesc(ctypes.Structure):
+    """struct mpnn_block_norm of include/mpnn_amd.h (field for field)."""
+    _fields_ = [
+        ("block", c_void_p), ("ldb", c_int64), ("residual", c_void_p), ("ldr", c_int64), ("gate", c_void_p), ("ldg", c_int64),
+        ("post_w", c_void_p), ("post_b", c_void_p), ("w", c_void_p), ("b", c_void_p),
+        ("N", c_int64), ("H", c_int32), ("dtype", c_int32), ("norm", c_int32), ("gate_kind", c_int32), ("post", c_int32),
+        ("eps", ctypes.c_float), ("residual_scale", ctypes.c_float), ("branch_scale", ctypes.c_float),
+        ("stream", c_void_p), ("lds", c_int64), ("normed", c_void_p), ("ldn", c_int64),
+        ("g_stream", c_void_p), ("ldgs", c_int64), ("g_normed", c_void_p), ("ldgn", c_int64),
+        ("g_block", c_void_p), ("ldgb", c_int64), ("g_residual", c_void_p), ("ldgr", c_int64),
+        ("g_gate", c_void_p), ("ldgg", c_int64),
+        ("g_post_w", c_void_p), ("g_post_b", c_void_p), ("g_w", c_void_p), ("g_b", c_void_p),
+        ("partial", c_void_p),
     ]
 
 
@@ -139,6 +155,9 @@ SIGNATURES = {
     "mpnn_halo_pack": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_void_p]),
     "mpnn_halo_unpack": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_int32,
                                    c_void_p]),
+    "mpnn_block_norm_partial_floats": (c_int64, [c_int64, c_int32, c_int32]),
+    "mpnn_block_norm_fwd": (c_int32, [ctypes.POINTER(BlockNormDesc), c_void_p]),
+    "mpnn_block_norm_bwd": (c_int32, [ctypes.POINTER(BlockNormDesc), c_void_p]),
     "mpnn_segment_mean_fwd": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                         c_int32, c_int32, c_void_p]),
     "mpnn_segment_mean_bwd": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
