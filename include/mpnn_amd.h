@@ -30,7 +30,8 @@ extern "C" {
 
 typedef struct ihipStream_t* mpnn_stream_t; /* == hipStream_t */
 
-enum { MPNN_F32 = 0, MPNN_BF16 = 1, MPNN_U8 = 2 /* only as the kind of a GEMM epilogue multiplier */ };
+enum { MPNN_F32 = 0, MPNN_BF16 = 1, MPNN_U8 = 2 /* only as the kind of a GEMM epilogue multiplier */,
+       MPNN_I8 = 3 /* only as the kind of mpnn_linear_int8's rows */ };
 
 enum {
   MPNN_OK = 0,
@@ -40,7 +41,7 @@ enum {
   MPNN_E_CAPACITY = -4   /* an output array's stated capacity is too small */
 };
 
-#define MPNN_ABI_VERSION 18
+#define MPNN_ABI_VERSION 19
 
 /* Library self-description. */
 int32_t mpnn_abi_version(void);
@@ -625,6 +626,42 @@ typedef struct mpnn_block_norm {
 int64_t mpnn_block_norm_partial_floats(int64_t N, int32_t H, int32_t dtype);
 int32_t mpnn_block_norm_fwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
 int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Rows held in 8 bits, the product with 8-bit weights, and the weight gradient from 8-bit rows (no counterpart in the
+ * reference; they stand next to the products of its Linear calls, models/layers.py:104,140).
+ *
+ * A row x of K values is kept as whole numbers q in [-127, 127], one byte each, and one float scale:
+ *   top = max|x|, scale = top / 127, inv = 127 / top (one float rounding each), q = x * inv to the nearest, ties to even
+ * A row with top < 2^-100 counts as zeros (scale 0); a row that holds an infinity or a NaN has scale NaN and q = 0.
+ * 8-bit rows are ldq bytes apart, at least K rounded up to 16; what lies behind column K may be anything.
+ *
+ * mpnn_quantize_rows    X [N, K] (dtype, any row stride) -> Q [N, ldq] (16-byte aligned, ldq a multiple of 16; the
+ *   bytes behind K are written as zeros), scale [N].  1 <= K <= 8192.
+ * mpnn_relu_bits        bits [N][ceil(M / 32)] words: bit i of word w is set unless Y[n, 32 w + i] <= 0.
+ * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * (x_scale[n] * w_scale[m]) + bias[m]); the sum is exact.  x_dtype
+ *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits first, in the
+ *   workspace (mpnn_linear_int8_workspace_bytes, 16-byte aligned).  W [M, ldw] 8-bit rows with w_scale [M]; bias [M]
+ *   of y_dtype or NULL.  8-bit rows 16-byte aligned, strides multiples of 16; K <= 8192.
+ * mpnn_gemm_tn8         dW[M, K + K2] = sum_n (G * open)[n, :]^T [scale[n] Q[n, :] | scale2[n] Q2[n, :]]
+ *   G, dW, Gout of dtype; bits (mpnn_relu_bits of the layer's output) or NULL select the entries of G that count; Gout
+ *   (optional, [N, M]) receives G * open.  Q2, scale2: optional (K2 = 0).  8-bit rows 4-byte aligned; row strides at
+ *   most 2^21; in bfloat16 M and the row strides of G and Gout are even and 4-byte aligned.  Rows are added in a fixed
+ *   order through `scratch` (mpnn_gemm_tn8_scratch_floats).
+ * ------------------------------------------------------------------------- */
+int32_t mpnn_quantize_rows(const void* X, int64_t ldx, int32_t dtype, int64_t N, int32_t K, void* Q, int64_t ldq,
+                           float* scale, mpnn_stream_t stream);
+int32_t mpnn_relu_bits(const void* Y, int64_t ldy, int32_t dtype, int64_t N, int32_t M, void* bits,
+                       mpnn_stream_t stream);
+int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_t x_dtype);
+int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const float* x_scale, const void* W, int64_t ldw,
+                         const float* w_scale, const void* bias, void* Y, int64_t ldy, int32_t y_dtype, int64_t N,
+                         int32_t K, int32_t M, int32_t relu, void* workspace, mpnn_stream_t stream);
+int64_t mpnn_gemm_tn8_scratch_floats(int64_t N, int32_t M, int32_t K, int32_t K2, int32_t dtype);
+int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bits, const void* Q, int64_t ldq,
+                      const float* scale, int32_t K, const void* Q2, int64_t ldq2, const float* scale2, int32_t K2,
+                      void* dW, int64_t lddw, float* scratch, void* Gout, int64_t ldgo, int64_t N, int32_t M,
+                      mpnn_stream_t stream);
 
 #ifdef __cplusplus
 }

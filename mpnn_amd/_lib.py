@@ -14,7 +14,8 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 MPNN_F32 = 0
 MPNN_BF16 = 1
 MPNN_U8 = 2
-ABI_VERSION = 18
+MPNN_I8 = 3
+ABI_VERSION = 19
 
 LIB_PATH = os.environ.get("MPNN_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmpnn_amd.so")
 
@@ -158,6 +159,15 @@ SIGNATURES = {
     "mpnn_block_norm_partial_floats": (c_int64, [c_int64, c_int32, c_int32]),
     "mpnn_block_norm_fwd": (c_int32, [ctypes.POINTER(BlockNormDesc), c_void_p]),
     "mpnn_block_norm_bwd": (c_int32, [ctypes.POINTER(BlockNormDesc), c_void_p]),
+    "mpnn_quantize_rows": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
+    "mpnn_relu_bits": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p]),
+    "mpnn_linear_int8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    "mpnn_linear_int8": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                   c_int64, c_int32, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "mpnn_gemm_tn8_scratch_floats": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32]),
+    "mpnn_gemm_tn8": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_void_p,
+                                c_int64, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                c_int32, c_void_p]),
     "mpnn_segment_mean_fwd": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                         c_int32, c_int32, c_void_p]),
     "mpnn_segment_mean_bwd": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
@@ -231,6 +241,19 @@ def dtype_code(dtype) -> int:
     if dtype == torch.bfloat16:
         return MPNN_BF16
     raise TypeError(f"mpnn_amd supports float32 and bfloat16 features, got {dtype}")
+
+
+def rows_in_place(t):
+    """The matrix itself if the library can read its rows where they lie (unit column stride, rows that do not
+    overlap: an expanded matrix repeats its rows at stride 0), else a contiguous copy."""
+    if (t.size(1) == 1 or t.stride(1) == 1) and (t.size(0) <= 1 or t.stride(0) >= t.size(1)):
+        return t
+    return t.contiguous()
+
+
+def leading(t) -> int:
+    """Row stride of such a matrix in elements, 0 for None.  A single row may carry any stride(0)."""
+    return 0 if t is None else max(t.stride(0), t.size(1))
 
 
 def require_device(t, name: str) -> None:

@@ -10,8 +10,11 @@ anything else raises - there is no fallback to torch's library GEMMs.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
+from .rows8 import Rows8, gemm_tn8, quantize_rows, relu_bits
 
 _SCRATCH = {}
 
@@ -230,20 +233,128 @@ def _require(name, *ts) -> None:
     raise TypeError(f"dense.{name}: operands must share float32 or bfloat16, got {[t.dtype for t in ts]}")
 
 
+class _ProjectKept(torch.autograd.Function):
+    """project with x kept in 8 bits for the weight gradient."""
+
+    @staticmethod
+    def forward(ctx, x, w, rows):
+        if ctx.needs_input_grad[1]:
+            rows = quantize_rows(x) if rows is None else rows
+            ctx.save_for_backward(w, rows.values, rows.scale)
+        else:
+            ctx.save_for_backward(w, None, None)
+        return _kit(x.dtype)[0](x, w)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        w, values, scale = ctx.saved_tensors
+        g = _upstream(g)
+        gx = _kit(g.dtype)[0](g, w.t().contiguous()) if ctx.needs_input_grad[0] else None
+        gw = gemm_tn8(g, Rows8(values, scale)) if ctx.needs_input_grad[1] else None
+        return gx, gw, None
+
+
+class _UpdateKept(torch.autograd.Function):
+    """update with x and aggr kept in 8 bits for the weight gradient and the relu in bits."""
+
+    @staticmethod
+    def forward(ctx, x, aggr, w_out):
+        f = x.size(1)
+        wx, wa = w_out[:, :f], w_out[:, f:]
+        if x.dtype == torch.bfloat16:
+            wx, wa = wx.contiguous(), wa.contiguous()
+        y = _kit(x.dtype)[0](x, wx, aggr, wa, relu=True)
+        kept = (None,) * 4
+        if ctx.needs_input_grad[2]:
+            rx, ra = quantize_rows(x), quantize_rows(aggr)
+            kept = (rx.values, rx.scale, ra.values, ra.scale)
+        ctx.f = f
+        ctx.save_for_backward(w_out, relu_bits(y), *kept)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        w_out, bits, xv, xs, av, as_ = ctx.saved_tensors
+        f, need = ctx.f, ctx.needs_input_grad
+        gy = _upstream(gy)
+        gz = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device) if need[0] or need[1] else None
+        gx = ga = gw = None
+        if need[2]:
+            gw = gemm_tn8(gy, Rows8(xv, xs), Rows8(av, as_), bits=bits, g_out=gz)
+        else:
+            gz = _open_entries(gy, bits)
+        if need[0] or need[1]:
+            nt = _kit(gy.dtype)[0]
+            wt = w_out.t().contiguous()
+            gx = nt(gz, wt[:f]) if need[0] else None
+            ga = nt(gz, wt[f:]) if need[1] else None
+        return gx, ga, gw
+
+
+def _open_entries(g, bits):
+    """g where the relu is open, zeros elsewhere (the path without a weight gradient, whose kernel does it otherwise)."""
+    m = g.size(1)
+    shifts = torch.arange(32, dtype=torch.int32, device=g.device)
+    is_open = ((bits.unsqueeze(2) >> shifts) & 1).reshape(g.size(0), -1)[:, :m].bool()
+    return torch.where(is_open, g, torch.zeros((), dtype=g.dtype, device=g.device))
+
+
+def _upstream(g):
+    """An upstream gradient the kernels can read: rows in place, 16-byte aligned rows in bfloat16."""
+    g = _lib.rows_in_place(g)
+    if g.dtype == torch.bfloat16 and not bf16_ok(g):
+        g = g.clone(memory_format=torch.contiguous_format)
+    return g
+
+
+def _checkpoint(name, checkpoint, allowed_rows, *xs):
+    """The 8-bit rows a caller brings (or None): checks ``checkpoint`` and the widths the 8-bit form takes."""
+    rows = None
+    if isinstance(checkpoint, Rows8) and allowed_rows:
+        rows = checkpoint
+        if rows.shape != xs[0].shape or rows.device != xs[0].device:
+            raise ValueError(f"dense.{name}: the 8-bit rows are {tuple(rows.shape)} on {rows.device}, x is "
+                             f"{tuple(xs[0].shape)} on {xs[0].device}")
+    elif checkpoint != "int8":
+        raise ValueError(f'dense.{name}: checkpoint must be None or "int8"' + (" or x's Rows8" if allowed_rows else "")
+                         + f", got {checkpoint!r}")
+    for x in xs:
+        if x.dim() != 2 or not 1 <= x.size(1) <= ROWS8_MAX_WIDTH:
+            raise ValueError(f"dense.{name}: 8-bit rows are 1 to {ROWS8_MAX_WIDTH} wide, got {tuple(x.shape)}")
+    return rows
+
+
 @torch.compiler.disable
-def project(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+def project(x: torch.Tensor, w: torch.Tensor, checkpoint=None) -> torch.Tensor:
+    """x @ w^T.  ``checkpoint="int8"``: x waits for the backward in 8 bits (or ``checkpoint=quantize_rows(x)``, when those
+    rows are at hand), from which the weight gradient is taken; differentiable once."""
     _require("project", x, w)
     if x.dtype == torch.bfloat16:
         x, w = x.contiguous(), w.contiguous()
-    return _Project.apply(x, w)
+    if checkpoint is None:
+        return _Project.apply(x, w)
+    rows = _checkpoint("project", checkpoint, True, x)
+    if w.dim() != 2 or w.size(1) != x.size(1):
+        raise ValueError(f"dense.project: w must have shape [M, {x.size(1)}], got {tuple(w.shape)}")
+    return _ProjectKept.apply(x, w, rows)
 
 
 @torch.compiler.disable
-def update(x: torch.Tensor, aggr: torch.Tensor, w_out: torch.Tensor) -> torch.Tensor:
+def update(x: torch.Tensor, aggr: torch.Tensor, w_out: torch.Tensor, checkpoint=None) -> torch.Tensor:
+    """relu(x @ w_out[:, :F]^T + aggr @ w_out[:, F:]^T).  ``checkpoint="int8"``: x and aggr wait for the backward in 8
+    bits and the relu in one bit per entry; differentiable once."""
     _require("update", x, aggr, w_out)
     if x.dtype == torch.bfloat16:
         x, aggr = x.contiguous(), aggr.contiguous()
-    return _Update.apply(x, aggr, w_out)
+    if checkpoint is None:
+        return _Update.apply(x, aggr, w_out)
+    _checkpoint("update", checkpoint, False, x, aggr)
+    if x.size(0) != aggr.size(0) or w_out.dim() != 2 or w_out.size(1) != x.size(1) + aggr.size(1):
+        raise ValueError(f"dense.update: w_out must have shape [M, {x.size(1) + aggr.size(1)}] and aggr {x.size(0)} rows, "
+                         f"got {tuple(w_out.shape)} and {tuple(aggr.shape)}")
+    return _UpdateKept.apply(x, aggr, w_out)
 
 
 _ONES = {}

@@ -30,17 +30,6 @@ _DESC = struct.Struct("@PqPqPq" "PPPP" "qiiiii" "fff" "PqPq" "PqPq" "PqPqPq" "PP
 assert _DESC.size == ctypes.sizeof(_lib.BlockNormDesc)
 
 
-def _rows(t):
-    """``t`` itself if its rows can be read in place (unit column stride, rows that do not overlap), else a copy."""
-    if (t.size(1) == 1 or t.stride(1) == 1) and (t.size(0) <= 1 or t.stride(0) >= t.size(1)):
-        return t
-    return t.contiguous()
-
-
-def _ld(t) -> int:
-    return 0 if t is None else max(t.stride(0), t.size(1))
-
-
 def _p(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -55,13 +44,13 @@ def _desc(plan, block, residual, gate, post_w, post_b, w, b, stream=None, normed
     d = _lib.BlockNormDesc()
     by_rows = plan.gate_kind > 1
     _DESC.pack_into(
-        d, 0, block.data_ptr(), _ld(block), _p(residual), _ld(residual), _p(gate), _ld(gate) if by_rows else 0,
+        d, 0, block.data_ptr(), _lib.leading(block), _p(residual), _lib.leading(residual), _p(gate), _lib.leading(gate) if by_rows else 0,
         _p(post_w), _p(post_b), _p(w), _p(b),
         block.size(0), block.size(1), _lib.dtype_code(block.dtype), plan.norm, plan.gate_kind, plan.post,
         plan.eps, plan.rs, plan.bs,
-        _p(stream), _ld(stream), _p(normed), _ld(normed),
-        _p(g_stream), _ld(g_stream), _p(g_normed), _ld(g_normed),
-        _p(g_block), _ld(g_block), _p(g_residual), _ld(g_residual), _p(g_gate), _ld(g_gate) if by_rows else 0,
+        _p(stream), _lib.leading(stream), _p(normed), _lib.leading(normed),
+        _p(g_stream), _lib.leading(g_stream), _p(g_normed), _lib.leading(g_normed),
+        _p(g_block), _lib.leading(g_block), _p(g_residual), _lib.leading(g_residual), _p(g_gate), _lib.leading(g_gate) if by_rows else 0,
         _p(g_post_w), _p(g_post_b), _p(g_w), _p(g_b), _p(partial))
     return d
 
@@ -100,8 +89,8 @@ class _BlockNorm(torch.autograd.Function):
         g_normed = grads[-1] if plan.outputs != "stream" else None
         if g_stream is None and g_normed is None:
             return (None,) * 8
-        g_stream = None if g_stream is None else _rows(g_stream)
-        g_normed = None if g_normed is None else _rows(g_normed)
+        g_stream = None if g_stream is None else _lib.rows_in_place(g_stream)
+        g_normed = None if g_normed is None else _lib.rows_in_place(g_normed)
         lib = _lib.load()
         n, h = block.shape
         outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and ctx.needs_input_grad[1 + i] else None
@@ -130,7 +119,7 @@ def _gate_kind(gate, n: int, h: int):
     if gate.shape == (h,):
         return 1, gate.contiguous()
     if gate.shape == (n, h):
-        return 3, _rows(gate)
+        return 3, _lib.rows_in_place(gate)
     if gate.shape == (n, 1):
         return 2, gate.contiguous()
     if gate.shape == (1, h):
@@ -175,7 +164,7 @@ def block_norm(block: torch.Tensor, residual: torch.Tensor | None = None, *, nor
         _operand("gate", gate, block, gate.shape)
         plan.gate_kind, gate = _gate_kind(gate, n, h)
     c = lambda t: None if t is None else t.contiguous()
-    tensors = (_rows(block), None if residual is None else _rows(residual), gate, c(post_weight), c(post_bias), c(weight), c(bias))
+    tensors = (_lib.rows_in_place(block), None if residual is None else _lib.rows_in_place(residual), gate, c(post_weight), c(post_bias), c(weight), c(bias))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return _BlockNorm.apply(plan, *tensors)
     stream, normed = _forward(plan, *tensors)
