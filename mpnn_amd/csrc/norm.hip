@@ -11,10 +11,14 @@
 // nothing but the inputs is kept between the passes, and the recomputed rows are the forward's before rounding.
 //
 // Bound: memory.  Forward 2 rows read and 2 written (3 read with a full gate), backward 4 read and 2 written, no
-// value touched twice; the sums over a row are shuffles inside the LPR lanes that hold it (a power of two from 8 to
-// 64 lanes, or the 256 of a block for wide rows), so a row never leaves registers between load and store.  Sums over
-// rows (gradients of weights, biases and a channel gate) stay in registers while a block walks its rows, leave one
-// slab per block and are added by a second launch in block order: no atomics, the same bits on every run.
+// value touched twice.  A row lies in LPR lanes (8 to 512, a power of two) with four columns each, so that two dozen
+// registers hold a row's streams, the parameters and the column sums and 16 waves per CU keep the next row of every
+// stream on its way (eight columns per lane halved the waves: 2.13 instead of 1.17 ms for the backward of 4 M rows
+// of 128 in bfloat16).  Sums over a row are lane exchanges on the vector unit, across waves (LPR > 64) through LDS.
+// Sums over rows (gradients of weights, biases and a channel gate) stay in registers while a block walks its rows,
+// leave one slab per block and are added by a second launch in block order: no atomics, the same bits on every run.
+// Measured on 4 M rows of 128 in bfloat16 (RMS, norms on both sides, channel gate): forward 0.82 ms = 5.0 TB/s, backward
+// 1.17 ms = 5.2 TB/s; a copy of 2 GiB reaches 4.9 TB/s.
 #include "common.h"
 #include "rowio.h"
 
@@ -23,7 +27,12 @@ namespace {
 
 constexpr int kNormMaxH = 2048;
 constexpr int kNormSums = 5;            // post_w, post_b, w, b, channel gate
-constexpr int kNormBwdBlocks = 1024;    // 4 blocks of 256 threads per CU
+// Waves per SIMD that the register budget of each direction is held to, and the blocks launched for them: a block more
+// would run after the others.
+constexpr int kNormFwdWaves = 6;
+constexpr int kNormBwdWaves = 4;
+
+constexpr int norm_threads(int lpr) { return lpr > kBlock ? lpr : kBlock; }
 
 struct NormArgs {
   const void *block, *residual, *gate, *post_w, *post_b, *w, *b;
@@ -42,36 +51,87 @@ struct NormArgs {
   float eps, rs, bs;
 };
 
-// Sums of K values over the LPR lanes of a row.  LPR = 256: the block's four waves meet in `red` (K floats per wave,
-// two sets used in turn, so that one barrier per call is enough).
+// Lane exchanges inside a row without the LDS crossbar: v of the lane that differs in the given bits of the lane index
+// (1 and 2: within a quad; 4 and 8: mirrored within 8 and 16 lanes, which is as good where quads already hold equal
+// sums).
+template <int CTRL>
+__device__ __forceinline__ float dpp_of(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+
+// Sums of K values over the LPR lanes of a row.  LPR > 64: the row's waves meet in `red` (two sets used in turn, so that
+// one barrier per call is enough; every row of the block is at the same call).
 template <int LPR, int K>
 struct RowSum {
   float* red;
   int turn;
   __device__ __forceinline__ void operator()(float (&v)[K]) {
-    constexpr int W = LPR < 64 ? LPR : 64;
 #pragma unroll
-    for (int off = W / 2; off > 0; off >>= 1)
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], off, 64);
+    for (int k = 0; k < K; ++k) {
+      v[k] += dpp_of<0xb1>(v[k]);    // quad_perm [1, 0, 3, 2]
+      v[k] += dpp_of<0x4e>(v[k]);    // quad_perm [2, 3, 0, 1]
+      v[k] += dpp_of<0x141>(v[k]);   // row_half_mirror
+      if constexpr (LPR >= 16) v[k] += dpp_of<0x140>(v[k]);   // row_mirror
+      if constexpr (LPR >= 32) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[k]), __float_as_uint(v[k]), false, false);
+        v[k] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+      }
+      if constexpr (LPR >= 64) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]), __float_as_uint(v[k]), false, false);
+        v[k] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+      }
+    }
     if constexpr (LPR > 64) {
-      float* r = red + turn * (K * 4);
-      const int wave = threadIdx.x >> 6;
+      constexpr int W = LPR / 64;                    // waves of a row
+      float* r = red + turn * (K * 8);
+      const int wave = threadIdx.x >> 6;             // at most 8 in the block
       if ((threadIdx.x & 63) == 0)
 #pragma unroll
-        for (int k = 0; k < K; ++k) r[k * 4 + wave] = v[k];
+        for (int k = 0; k < K; ++k) r[k * 8 + wave] = v[k];
       __syncthreads();
+      const int first = wave / W * W;
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[k] = (r[k * 4] + r[k * 4 + 1]) + (r[k * 4 + 2] + r[k * 4 + 3]);
+      for (int k = 0; k < K; ++k) {
+        float t = r[k * 8 + first];
+#pragma unroll
+        for (int w = 1; w < W; ++w) t += r[k * 8 + first + w];
+        v[k] = t;
+      }
       turn ^= 1;
     }
   }
 };
 
-// The columns a lane owns: vector v of NV covers columns (v * LPR + lane) * VEC and the VEC - 1 after it.
+// Two floats to packed bfloat16, nearest even (one instruction).
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, bf16x2_t));
+}
+
+// VEC columns of T at a time: 16 bytes in float32, 8 in bfloat16, or one column.
+template <typename T, int VEC>
+struct NormIO : RowIO<T, VEC> {};
+template <>
+struct NormIO<bf16_t, 4> {
+  typedef uint2 Raw;
+  static __device__ __forceinline__ Raw load_raw(const bf16_t* p) { return *reinterpret_cast<const uint2*>(p); }
+  static __device__ __forceinline__ void unpack(const Raw& t, float (&v)[4]) {
+    v[0] = __uint_as_float(t.x << 16); v[1] = __uint_as_float(t.x & 0xffff0000u);
+    v[2] = __uint_as_float(t.y << 16); v[3] = __uint_as_float(t.y & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+  }
+};
+
+// The columns a lane owns: vector v of NV covers columns (v * LPR + lane) * VEC and the VEC - 1 after it.  Raw: the
+// lane's share of a row as it lies in memory, which a row that is on its way takes less registers for.
 template <typename T, int VEC, int NV, int LPR>
 struct Lane {
   static constexpr int C = VEC * NV;
+  typedef NormIO<T, VEC> IO;
+  struct Raw { typename IO::Raw v[NV]; };
   int col[NV];
   bool in[NV];
   __device__ __forceinline__ void init(int lane, int H) {
@@ -79,37 +139,76 @@ struct Lane {
     for (int v = 0; v < NV; ++v) {
       const int c = (v * LPR + lane) * VEC;
       in[v] = c < H;              // widths are multiples of VEC on this path: a vector is in or out
-      col[v] = in[v] ? c : 0;
+      col[v] = in[v] ? c : 0;     // lanes past the row load its first vector and count it as zeros
     }
   }
-  __device__ __forceinline__ void load(const void* base, int64_t off, float (&x)[C]) const {
+  __device__ __forceinline__ void fetch(const void* base, int64_t off, Raw& r) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) r.v[v] = IO::load_raw(static_cast<const T*>(base) + off + col[v]);
+  }
+  __device__ __forceinline__ void unpack(const Raw& r, float (&x)[C]) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float t[VEC];
+      IO::unpack(r.v[v], t);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) t[k] = 0.f;
-      if (in[v]) RowIO<T, VEC>::load(static_cast<const T*>(base) + off + col[v], t);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[v * VEC + k] = t[k];
+      for (int k = 0; k < VEC; ++k) x[v * VEC + k] = in[v] ? t[k] : 0.f;
     }
   }
   __device__ __forceinline__ void store(void* base, int64_t off, const float (&x)[C]) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      if (!in[v]) continue;
+      T* p = static_cast<T*>(base) + off + col[v];
       float t[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) t[k] = x[v * VEC + k];
-      if (in[v]) RowIO<T, VEC>::store(static_cast<T*>(base) + off + col[v], t);
+      IO::store(p, t);
     }
   }
   // a column vector, `other` where there is none
   __device__ __forceinline__ void vector(const void* base, float other, float (&x)[C]) const {
-    if (base) load(base, 0, x);
-    else
+    if (base) {
+      Raw r;
+      fetch(base, 0, r);
+      unpack(r, x);
+    } else
 #pragma unroll
       for (int c = 0; c < C; ++c) x[c] = other;
   }
 };
+
+// What a row's tensors hold, on its way from memory.  One row of each stream is always in flight while the one before
+// it is worked on.
+template <typename L, typename T, bool BACKWARD>
+struct RowData {
+  typename L::Raw block, residual, gate, g_stream, g_normed;
+  T row_gate;
+  __device__ __forceinline__ void fetch(const NormArgs& a, const L& lane, int64_t row) {
+    lane.fetch(a.block, row * a.ldb, block);
+    if (a.residual) lane.fetch(a.residual, row * a.ldr, residual);
+    if (a.gate_kind == MPNN_GATE_FULL) lane.fetch(a.gate, row * a.ldg, gate);
+    if (a.gate_kind == MPNN_GATE_ROW) row_gate = static_cast<const T*>(a.gate)[row * a.ldg];
+    if constexpr (BACKWARD) {
+      if (a.g_stream) lane.fetch(a.g_stream, row * a.ldgs, g_stream);
+      if (a.g_normed) lane.fetch(a.g_normed, row * a.ldgn, g_normed);
+    }
+  }
+};
+
+// The gate of a row times branch_scale; gch holds the channel gate (ones without one).
+template <typename L, typename T, int C, typename D>
+__device__ __forceinline__ void gate_of(const NormArgs& a, const L& lane, const D& d, const float (&gch)[C], float (&g)[C]) {
+  if (a.gate_kind == MPNN_GATE_FULL) {
+    lane.unpack(d.gate, g);
+#pragma unroll
+    for (int c = 0; c < C; ++c) g[c] *= a.bs;
+  } else {
+    const float one = a.gate_kind == MPNN_GATE_ROW ? a.bs * scalar_to_f32(d.row_gate) : a.bs;
+#pragma unroll
+    for (int c = 0; c < C; ++c) g[c] = gch[c] * one;
+  }
+}
 
 // v -> hat in place, returns inv.  Columns past H hold zeros before and after.
 template <typename L, int LPR, int C, int VEC>
@@ -128,87 +227,110 @@ __device__ __forceinline__ float normalize(float (&v)[C], const L& lane, bool la
 #pragma unroll
   for (int c = 0; c < C; ++c) q[0] = fmaf(v[c], v[c], q[0]);
   sum(q);
-  const float inv = 1.f / sqrtf(q[0] * inv_h + eps);
+  const float inv = rsqrtf(q[0] * inv_h + eps);
 #pragma unroll
   for (int c = 0; c < C; ++c) v[c] *= inv;
   return inv;
 }
 
-template <typename T, int VEC, int NV, int LPR>
-__global__ void __launch_bounds__(kBlock) k_block_norm_fwd(NormArgs a) {
+// FORM: bit 0 the layer norm, bit 1 a norm of the block too; -1: as the arguments say (the column-by-column shapes)
+template <int FORM>
+__device__ __forceinline__ bool is_layer(const NormArgs& a) { return FORM < 0 ? a.layer != 0 : (FORM & 1) != 0; }
+template <int FORM>
+__device__ __forceinline__ bool is_post(const NormArgs& a) { return FORM < 0 ? a.post != 0 : (FORM & 2) != 0; }
+
+template <typename T, int VEC, int NV, int LPR, int FORM>
+__global__ void __launch_bounds__(norm_threads(LPR), kNormFwdWaves) k_block_norm_fwd(NormArgs a) {
   typedef Lane<T, VEC, NV, LPR> L;
-  constexpr int C = L::C;
-  __shared__ float red[8];
+  constexpr int C = L::C, THREADS = norm_threads(LPR), ROWS = THREADS / LPR;   // rows of a block at a time
+  __shared__ float red[16];
   L lane;
   lane.init(threadIdx.x % LPR, a.H);
   RowSum<LPR, 1> sum{red, 0};
   const float inv_h = 1.f / (float)a.H;
+  const bool layer = is_layer<FORM>(a), post = is_post<FORM>(a);
   float pw[C], pb[C], w[C], b[C], gch[C];
   lane.vector(a.post_w, 1.f, pw);
   lane.vector(a.post_b, 0.f, pb);
   lane.vector(a.w, 1.f, w);
   lane.vector(a.b, 0.f, b);
   lane.vector(a.gate_kind == MPNN_GATE_CHANNEL ? a.gate : nullptr, 1.f, gch);
-  const int64_t step = (int64_t)gridDim.x * (kBlock / LPR);
-  for (int64_t row = (int64_t)blockIdx.x * (kBlock / LPR) + threadIdx.x / LPR; row < a.N; row += step) {
-    float n[C], s[C];
-    lane.load(a.block, row * a.ldb, n);
-    if (a.residual) lane.load(a.residual, row * a.ldr, s);
-    else
-#pragma unroll
-      for (int c = 0; c < C; ++c) s[c] = 0.f;
-    float g[C];
-    if (a.gate_kind == MPNN_GATE_FULL) lane.load(a.gate, row * a.ldg, g);
-    else {
-      const float one = a.gate_kind == MPNN_GATE_ROW ? scalar_to_f32(static_cast<const T*>(a.gate)[row * a.ldg]) : 1.f;
-#pragma unroll
-      for (int c = 0; c < C; ++c) g[c] = gch[c] * one;
-    }
-    if (a.post) {
-      normalize<L, LPR, C, VEC>(n, lane, a.layer, inv_h, a.eps, sum);
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR;
+  // rows of several waves meet at barriers: a row past the end goes along, reads the last row and leaves nothing
+  int64_t turns = a.N > row ? (a.N - row + step - 1) / step : 0;
+  if constexpr (LPR > 64) turns = (a.N - (int64_t)blockIdx.x * ROWS + step - 1) / step;
+  RowData<L, T, false> next, now;
+  if (turns > 0) next.fetch(a, lane, row < a.N ? row : a.N - 1);
+  for (; turns > 0; --turns, row += step) {
+    now = next;
+    const bool live = LPR <= 64 || row < a.N;
+    if (turns > 1) next.fetch(a, lane, row + step < a.N ? row + step : a.N - 1);
+    float n[C], s[C], g[C];
+    lane.unpack(now.block, n);
+    gate_of<L, T, C>(a, lane, now, gch, g);
+    if (post) {
+      normalize<L, LPR, C, VEC>(n, lane, layer, inv_h, a.eps, sum);
 #pragma unroll
       for (int c = 0; c < C; ++c) n[c] = fmaf(n[c], pw[c], pb[c]);
     }
+    if (a.residual) {
+      lane.unpack(now.residual, s);
 #pragma unroll
-    for (int c = 0; c < C; ++c) s[c] = fmaf(a.bs * g[c], n[c], a.rs * s[c]);
-    if (a.stream) lane.store(a.stream, row * a.lds, s);
+      for (int c = 0; c < C; ++c) s[c] = fmaf(g[c], n[c], a.rs * s[c]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) s[c] = g[c] * n[c];
+    }
+    if (a.stream && live) lane.store(a.stream, row * a.lds, s);
     if (a.normed) {
-      normalize<L, LPR, C, VEC>(s, lane, a.layer, inv_h, a.eps, sum);
+      normalize<L, LPR, C, VEC>(s, lane, layer, inv_h, a.eps, sum);
 #pragma unroll
       for (int c = 0; c < C; ++c) s[c] = fmaf(s[c], w[c], b[c]);
-      lane.store(a.normed, row * a.ldn, s);
+      if (live) lane.store(a.normed, row * a.ldn, s);
     }
   }
 }
 
 // Gradient of v from gh = gy * w and hat, inv of the forward.
 template <typename L, int LPR, int C, int VEC>
-__device__ __forceinline__ void norm_backward(float (&gh)[C], const float (&hat)[C], float inv, const L& lane, bool layer,
-                                              float inv_h, RowSum<LPR, 2>& sum) {
-  float s[2] = {0.f, 0.f};
+__device__ __forceinline__ void norm_backward(float (&gh)[C], const float (&hat)[C], float inv, bool layer, float inv_h,
+                                              RowSum<LPR, 1>& sum, RowSum<LPR, 2>& sum2) {
+  float m0 = 0.f, m1;
+  if (layer) {
+    float s[2] = {0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    s[0] += gh[c];                      // columns past H hold zeros
-    s[1] = fmaf(gh[c], hat[c], s[1]);
+    for (int c = 0; c < C; ++c) {       // columns past H hold zeros
+      s[0] += gh[c];
+      s[1] = fmaf(gh[c], hat[c], s[1]);
+    }
+    sum2(s);
+    m0 = s[0] * inv_h;
+    m1 = s[1] * inv_h;
+  } else {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) s[0] = fmaf(gh[c], hat[c], s[0]);
+    sum(s);
+    m1 = s[0] * inv_h;
   }
-  sum(s);
-  const float m0 = layer ? s[0] * inv_h : 0.f, m1 = s[1] * inv_h;
 #pragma unroll
-  for (int c = 0; c < C; ++c) gh[c] = inv * (gh[c] - m0 - hat[c] * m1);
+  for (int c = 0; c < C; ++c) gh[c] = inv * ((layer ? gh[c] - m0 : gh[c]) - hat[c] * m1);
 }
 
-template <typename T, int VEC, int NV, int LPR>
-__global__ void __launch_bounds__(kBlock) k_block_norm_bwd(NormArgs a) {
+template <typename T, int VEC, int NV, int LPR, int FORM>
+__global__ void __launch_bounds__(norm_threads(LPR), kNormBwdWaves) k_block_norm_bwd(NormArgs a) {
   typedef Lane<T, VEC, NV, LPR> L;
-  constexpr int C = L::C;
-  __shared__ float red[8];
-  __shared__ float red2[16];
-  __shared__ float col[kBlock * C];
+  constexpr int C = L::C, THREADS = norm_threads(LPR), ROWS = THREADS / LPR;   // rows of a block at a time
+  __shared__ float red[16];
+  __shared__ float red2[32];
+  __shared__ float col[THREADS * C];
   L lane;
   lane.init(threadIdx.x % LPR, a.H);
   RowSum<LPR, 1> sum{red, 0};
   RowSum<LPR, 2> sum2{red2, 0};
   const float inv_h = 1.f / (float)a.H;
+  const bool layer = is_layer<FORM>(a), post = is_post<FORM>(a);
   float pw[C], pb[C], w[C], gch[C];
   lane.vector(a.post_w, 1.f, pw);
   lane.vector(a.post_b, 0.f, pb);
@@ -219,48 +341,63 @@ __global__ void __launch_bounds__(kBlock) k_block_norm_bwd(NormArgs a) {
   for (int k = 0; k < kNormSums; ++k)
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[k][c] = 0.f;
-  const int64_t step = (int64_t)gridDim.x * (kBlock / LPR);
-  for (int64_t row = (int64_t)blockIdx.x * (kBlock / LPR) + threadIdx.x / LPR; row < a.N; row += step) {
-    float n[C], s[C], gs[C], gu[C], g[C];
-    lane.load(a.block, row * a.ldb, n);
-    if (a.residual) lane.load(a.residual, row * a.ldr, s);
-    else
-#pragma unroll
-      for (int c = 0; c < C; ++c) s[c] = 0.f;
-    if (a.gate_kind == MPNN_GATE_FULL) lane.load(a.gate, row * a.ldg, g);
-    else {
-      const float one = a.gate_kind == MPNN_GATE_ROW ? scalar_to_f32(static_cast<const T*>(a.gate)[row * a.ldg]) : 1.f;
-#pragma unroll
-      for (int c = 0; c < C; ++c) g[c] = gch[c] * one;
-    }
-    if (a.g_stream) lane.load(a.g_stream, row * a.ldgs, gs);
-    else
-#pragma unroll
-      for (int c = 0; c < C; ++c) gs[c] = 0.f;
-    float hat1[C], inv1 = 0.f;
-    if (a.post) {
-      inv1 = normalize<L, LPR, C, VEC>(n, lane, a.layer, inv_h, a.eps, sum);
+  const bool biases = a.slot[1] >= 0 || a.slot[3] >= 0;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR;
+  // rows of several waves meet at barriers: a row past the end goes along, reads the last row and leaves nothing
+  int64_t turns = a.N > row ? (a.N - row + step - 1) / step : 0;
+  if constexpr (LPR > 64) turns = (a.N - (int64_t)blockIdx.x * ROWS + step - 1) / step;
+  RowData<L, T, true> next, now;
+  if (turns > 0) next.fetch(a, lane, row < a.N ? row : a.N - 1);
+  for (; turns > 0; --turns, row += step) {
+    now = next;
+    const bool live = LPR <= 64 || row < a.N;
+    if (turns > 1) next.fetch(a, lane, row + step < a.N ? row + step : a.N - 1);
+    float n[C], s[C], gs[C], gu[C], g[C], hat1[C], inv1 = 0.f;
+    lane.unpack(now.block, n);
+    gate_of<L, T, C>(a, lane, now, gch, g);
+    if (post) {
+      inv1 = normalize<L, LPR, C, VEC>(n, lane, layer, inv_h, a.eps, sum);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         hat1[c] = n[c];
         n[c] = fmaf(n[c], pw[c], pb[c]);
       }
-    } else {
+    }
+    if (a.g_stream) lane.unpack(now.g_stream, gs);
+    else
 #pragma unroll
-      for (int c = 0; c < C; ++c) hat1[c] = 0.f;
+      for (int c = 0; c < C; ++c) gs[c] = 0.f;
+    if constexpr (LPR > 64) {
+      if (!live)
+#pragma unroll
+        for (int c = 0; c < C; ++c) gs[c] = 0.f;
     }
     if (a.g_normed) {
-      lane.load(a.g_normed, row * a.ldgn, gu);
+      if (a.residual) {
+        lane.unpack(now.residual, s);
 #pragma unroll
-      for (int c = 0; c < C; ++c) s[c] = fmaf(a.bs * g[c], n[c], a.rs * s[c]);
-      const float inv2 = normalize<L, LPR, C, VEC>(s, lane, a.layer, inv_h, a.eps, sum);
+        for (int c = 0; c < C; ++c) s[c] = fmaf(g[c], n[c], a.rs * s[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[c] = g[c] * n[c];
+      }
+      const float inv2 = normalize<L, LPR, C, VEC>(s, lane, layer, inv_h, a.eps, sum);
+      lane.unpack(now.g_normed, gu);
+      if constexpr (LPR > 64) {
+        if (!live)
+#pragma unroll
+          for (int c = 0; c < C; ++c) gu[c] = 0.f;
+      }
+      if (biases)
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[3][c] += gu[c];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         acc[2][c] = fmaf(gu[c], s[c], acc[2][c]);
-        acc[3][c] += gu[c];
         gu[c] *= w[c];
       }
-      norm_backward<L, LPR, C, VEC>(gu, s, inv2, lane, a.layer, inv_h, sum2);
+      norm_backward<L, LPR, C, VEC>(gu, s, inv2, layer, inv_h, sum, sum2);
 #pragma unroll
       for (int c = 0; c < C; ++c) gs[c] += lane.in[c / VEC] ? gu[c] : 0.f;
     }
@@ -268,33 +405,38 @@ __global__ void __launch_bounds__(kBlock) k_block_norm_bwd(NormArgs a) {
     if (a.g_residual) {
 #pragma unroll
       for (int c = 0; c < C; ++c) gu[c] = a.rs * gs[c];
-      lane.store(a.g_residual, row * a.ldgr, gu);
+      if (live) lane.store(a.g_residual, row * a.ldgr, gu);
+    }
+    if (a.gate_kind != MPNN_GATE_NONE) {   // gradient of the gate
+#pragma unroll
+      for (int c = 0; c < C; ++c) gu[c] = gs[c] * (a.bs * n[c]);
+      if (a.gate_kind == MPNN_GATE_CHANNEL) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[4][c] += gu[c];
+      } else if (a.g_gate && a.gate_kind == MPNN_GATE_FULL) {
+        if (live) lane.store(a.g_gate, row * a.ldgg, gu);
+      } else if (a.g_gate) {
+        float t[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) t[0] += lane.in[c / VEC] ? gu[c] : 0.f;
+        sum(t);
+        if (threadIdx.x % LPR == 0 && live) static_cast<T*>(a.g_gate)[row * a.ldgg] = f32_to_scalar<T>(t[0]);
+      }
     }
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      gs[c] *= a.bs;
-      gu[c] = gs[c] * n[c];            // gradient of the gate
-      gs[c] *= g[c];                   // gradient of n
-      acc[4][c] += gu[c];
-    }
-    if (a.g_gate && a.gate_kind == MPNN_GATE_FULL) lane.store(a.g_gate, row * a.ldgg, gu);
-    if (a.g_gate && a.gate_kind == MPNN_GATE_ROW) {
-      float t[1] = {0.f};
+    for (int c = 0; c < C; ++c) gs[c] *= g[c];   // gradient of n
+    if (post) {
+      if (biases)
 #pragma unroll
-      for (int c = 0; c < C; ++c) t[0] += lane.in[c / VEC] ? gu[c] : 0.f;
-      sum(t);
-      if (threadIdx.x % LPR == 0) static_cast<T*>(a.g_gate)[row * a.ldgg] = f32_to_scalar<T>(t[0]);
-    }
-    if (a.post) {
+        for (int c = 0; c < C; ++c) acc[1][c] += gs[c];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         acc[0][c] = fmaf(gs[c], hat1[c], acc[0][c]);
-        acc[1][c] += gs[c];
         gs[c] *= pw[c];
       }
-      if (a.g_block) norm_backward<L, LPR, C, VEC>(gs, hat1, inv1, lane, a.layer, inv_h, sum2);
+      if (a.g_block) norm_backward<L, LPR, C, VEC>(gs, hat1, inv1, layer, inv_h, sum, sum2);
     }
-    if (a.g_block) lane.store(a.g_block, row * a.ldgb, gs);
+    if (a.g_block && live) lane.store(a.g_block, row * a.ldgb, gs);
   }
   // column sums of the block: the row groups meet in LDS, group 0 first
 #pragma unroll
@@ -305,10 +447,10 @@ __global__ void __launch_bounds__(kBlock) k_block_norm_bwd(NormArgs a) {
     for (int c = 0; c < C; ++c) col[threadIdx.x * C + c] = acc[k][c];
     __syncthreads();
     float* out = a.partial + ((int64_t)blockIdx.x * a.n_sums + a.slot[k]) * a.H;
-    for (int j = threadIdx.x; j < a.H; j += kBlock) {
+    for (int j = threadIdx.x; j < a.H; j += THREADS) {
       const int vec = j / VEC, v = vec / LPR, l = vec - v * LPR;
       float t = 0.f;
-      for (int g = 0; g < kBlock / LPR; ++g) t += col[(g * LPR + l) * C + v * VEC + (j - vec * VEC)];
+      for (int g = 0; g < ROWS; ++g) t += col[(g * LPR + l) * C + v * VEC + (j - vec * VEC)];
       out[j] = t;
     }
   }
@@ -320,88 +462,85 @@ struct NormSumArgs {
   int32_t n_sums, H, blocks;
 };
 
-// out[slot][j] = sum over blocks of partial[block][slot][j]: wave w of a block adds blocks w, w + 4, .. for 64
-// consecutive sums, then the four wave sums are added in wave order.
+// out[slot][j] = sum over blocks of partial[block][slot][j].  A block takes 16 consecutive sums, 16 threads each: thread
+// t of a sum adds blocks t, t + 16, .., then the 16 meet in LDS in that order (a wave per 64 sums walked the 768 slabs
+// in 13 to 19 us).
 template <typename T>
 __global__ void __launch_bounds__(kBlock) k_block_norm_sums(NormSumArgs a) {
   __shared__ float red[kBlock];
   const int total = a.n_sums * a.H;
-  const int o = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int i = blockIdx.x * 64 + o;
+  const int o = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int i = blockIdx.x * 16 + o;
   float s = 0.f;
   if (i < total) {
-#pragma unroll 8
-    for (int b = g; b < a.blocks; b += kBlock / 64) s += a.partial[(int64_t)b * total + i];
+#pragma unroll 16
+    for (int b = g; b < a.blocks; b += 16) s += a.partial[(int64_t)b * total + i];
   }
   red[threadIdx.x] = s;
   __syncthreads();
   if (g == 0 && i < total) {
-    const float t = (red[o] + red[64 + o]) + (red[128 + o] + red[192 + o]);
+    float t = red[o];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) t += red[k * 16 + o];
     const int k = i / a.H;
     static_cast<T*>(a.out[k])[i - k * a.H] = f32_to_scalar<T>(t);
   }
 }
 
-// How a row is spread: LPR lanes with NV vectors of VEC columns each.
-struct NormShape { int vec, nv, lpr; };
-
-// Whole 16-byte vectors: the smallest power of two of lanes that holds the row once; rows of more than 64 vectors
-// take two per lane in float32 and a block of 256 lanes beyond that.  Other widths and alignments: one column per
-// vector, up to 8 per lane.
-NormShape norm_shape(int H, bool wide, bool bf16) {
-  const int vec = wide ? (bf16 ? 8 : 4) : 1;
-  const int nvec = H / vec;
-  if (wide) {
-    for (int lpr = 8; lpr <= 64; lpr *= 2)
-      if (nvec <= lpr) return {vec, 1, lpr};
-    if (!bf16 && nvec <= 128) return {vec, 2, 64};
-    return {vec, nvec <= 256 ? 1 : 2, 256};
-  }
-  if (nvec <= 16) return {1, 1, 16};
-  for (int nv = 1; nv <= 8; nv *= 2)
-    if (nvec <= 64 * nv) return {1, nv, 64};
-  return {1, nvec <= 1024 ? 4 : 8, 256};
+// Lanes of a row: the smallest power of two that holds it with four columns per lane, in one vector (`wide`: width,
+// addresses and strides allow 16 bytes in float32, 8 in bfloat16) or column by column.
+int norm_lanes(int H, bool wide) {
+  int lpr = wide ? 8 : 16;
+  while (lpr * 4 < H) lpr *= 2;
+  return !wide && lpr == 32 ? 64 : lpr;
 }
 
 // Blocks of the backward: at least four rows per row group, so that the slabs of column sums stay small next to the
 // rows.
-int norm_bwd_blocks(int64_t N, const NormShape& s) {
-  const int64_t per = 4 * (kBlock / s.lpr);
+int norm_bwd_blocks(int64_t N, int lpr) {
+  const int64_t per = 4 * (norm_threads(lpr) / lpr);
   const int64_t b = (N + per - 1) / per;
-  return (int)(b > kNormBwdBlocks ? kNormBwdBlocks : b);
+  const int most = 256 * 4 * kNormBwdWaves / (norm_threads(lpr) / 64);
+  return (int)(b > most ? most : b);
+}
+
+template <typename T, int VEC, int NV, int LPR, int FORM>
+void launch_form(const NormArgs& a, bool backward, int blocks, hipStream_t stream) {
+  if (backward) k_block_norm_bwd<T, VEC, NV, LPR, FORM><<<blocks, norm_threads(LPR), 0, stream>>>(a);
+  else k_block_norm_fwd<T, VEC, NV, LPR, FORM><<<blocks, norm_threads(LPR), 0, stream>>>(a);
 }
 
 template <typename T, int VEC, int NV, int LPR>
 void launch_norm(const NormArgs& a, bool backward, int blocks, hipStream_t stream) {
-  if (backward) k_block_norm_bwd<T, VEC, NV, LPR><<<blocks, kBlock, 0, stream>>>(a);
-  else k_block_norm_fwd<T, VEC, NV, LPR><<<blocks, kBlock, 0, stream>>>(a);
+  if constexpr (VEC == 1) {
+    launch_form<T, VEC, NV, LPR, -1>(a, backward, blocks, stream);
+  } else {
+    const int form = (a.layer ? 1 : 0) | (a.post ? 2 : 0);
+    if (form == 0) launch_form<T, VEC, NV, LPR, 0>(a, backward, blocks, stream);
+    else if (form == 1) launch_form<T, VEC, NV, LPR, 1>(a, backward, blocks, stream);
+    else if (form == 2) launch_form<T, VEC, NV, LPR, 2>(a, backward, blocks, stream);
+    else launch_form<T, VEC, NV, LPR, 3>(a, backward, blocks, stream);
+  }
 }
 
 template <typename T>
-bool dispatch_norm(const NormArgs& a, const NormShape& s, bool backward, int blocks, hipStream_t stream) {
-  constexpr int V = sizeof(T) == 2 ? 8 : 4;
-  if (s.vec == V) {
-    if (s.nv == 1 && s.lpr == 8) launch_norm<T, V, 1, 8>(a, backward, blocks, stream);
-    else if (s.nv == 1 && s.lpr == 16) launch_norm<T, V, 1, 16>(a, backward, blocks, stream);
-    else if (s.nv == 1 && s.lpr == 32) launch_norm<T, V, 1, 32>(a, backward, blocks, stream);
-    else if (s.nv == 1 && s.lpr == 64) launch_norm<T, V, 1, 64>(a, backward, blocks, stream);
-    else if (s.nv == 1 && s.lpr == 256) launch_norm<T, V, 1, 256>(a, backward, blocks, stream);
-    else if constexpr (V == 4) {
-      if (s.nv == 2 && s.lpr == 64) launch_norm<T, V, 2, 64>(a, backward, blocks, stream);
-      else if (s.nv == 2 && s.lpr == 256) launch_norm<T, V, 2, 256>(a, backward, blocks, stream);
-      else return false;
-    } else return false;
-    return true;
+bool dispatch_norm(const NormArgs& a, bool wide, int lpr, bool backward, int blocks, hipStream_t stream) {
+#define MPNN_NORM(LPR)                                                          \
+  if (lpr == LPR) {                                                             \
+    if (wide) launch_norm<T, 4, 1, LPR>(a, backward, blocks, stream);           \
+    else if constexpr (LPR != 8 && LPR != 32) launch_norm<T, 1, 4, LPR>(a, backward, blocks, stream); \
+    else return false;                                                          \
+    return true;                                                                \
   }
-  if (s.lpr == 16 && s.nv == 1) launch_norm<T, 1, 1, 16>(a, backward, blocks, stream);
-  else if (s.lpr == 64 && s.nv == 1) launch_norm<T, 1, 1, 64>(a, backward, blocks, stream);
-  else if (s.lpr == 64 && s.nv == 2) launch_norm<T, 1, 2, 64>(a, backward, blocks, stream);
-  else if (s.lpr == 64 && s.nv == 4) launch_norm<T, 1, 4, 64>(a, backward, blocks, stream);
-  else if (s.lpr == 64 && s.nv == 8) launch_norm<T, 1, 8, 64>(a, backward, blocks, stream);
-  else if (s.lpr == 256 && s.nv == 4) launch_norm<T, 1, 4, 256>(a, backward, blocks, stream);
-  else if (s.lpr == 256 && s.nv == 8) launch_norm<T, 1, 8, 256>(a, backward, blocks, stream);
-  else return false;
-  return true;
+  MPNN_NORM(8)
+  MPNN_NORM(16)
+  MPNN_NORM(32)
+  MPNN_NORM(64)
+  MPNN_NORM(128)
+  MPNN_NORM(256)
+  MPNN_NORM(512)
+#undef MPNN_NORM
+  return false;
 }
 
 // Checks what both directions share and fills the kernel's arguments; `wide`: every row of every operand can move as
@@ -418,16 +557,16 @@ int32_t norm_args(const char* who, const mpnn_block_norm* d, bool backward, Norm
   if (rows && !d->block) return fail(MPNN_E_INVALID, "%s: null pointer argument", who);
   if ((d->gate_kind != MPNN_GATE_NONE) != (d->gate != nullptr) && (rows || d->gate))
     return fail(MPNN_E_INVALID, "%s: gate and its kind disagree", who);
-  const int H = d->H, vec = d->dtype == MPNN_BF16 ? 8 : 4;
-  wide = H % vec == 0;
+  const int H = d->H, vec_bytes = d->dtype == MPNN_BF16 ? 8 : 16;
+  wide = H % 4 == 0;
   bool ok = true;
   auto row = [&](const void* p, int64_t ld) {
     if (!p) return;
     if (ld < H) ok = false;
-    if (((uintptr_t)p & 15) || ld % vec) wide = false;
+    if ((uintptr_t)p % vec_bytes || ld % 4) wide = false;
   };
   auto vector = [&](const void* p) {
-    if (p && ((uintptr_t)p & 15)) wide = false;
+    if (p && (uintptr_t)p % vec_bytes) wide = false;
   };
   row(d->block, d->ldb);
   row(d->residual, d->ldr);
@@ -475,22 +614,22 @@ int32_t mpnn_block_norm_fwd(const mpnn_block_norm* d, mpnn_stream_t stream) {
   if (!d->stream && !d->normed) return fail(MPNN_E_INVALID, "mpnn_block_norm_fwd: no output");
   a.stream = d->stream; a.lds = d->lds; a.normed = d->normed; a.ldn = d->ldn;
   const bool bf16 = d->dtype == MPNN_BF16;
-  const NormShape s = norm_shape(d->H, wide, bf16);
-  const int64_t need = (d->N + kBlock / s.lpr - 1) / (kBlock / s.lpr);
-  const int blocks = (int)(need > kMaxBlocks ? kMaxBlocks : need);
-  const bool known = bf16 ? dispatch_norm<bf16_t>(a, s, false, blocks, stream) : dispatch_norm<float>(a, s, false, blocks, stream);
+  const int lpr = norm_lanes(d->H, wide), rows = norm_threads(lpr) / lpr;
+  const int64_t need = (d->N + rows - 1) / rows, most = 256 * 4 * kNormFwdWaves / (norm_threads(lpr) / 64);
+  const int blocks = (int)(need > most ? most : need);
+  const bool known = bf16 ? dispatch_norm<bf16_t>(a, wide, lpr, false, blocks, stream)
+                          : dispatch_norm<float>(a, wide, lpr, false, blocks, stream);
   if (!known) return fail(MPNN_E_INVALID, "mpnn_block_norm_fwd: no kernel for H=%d", d->H);
   MPNN_LAUNCH_CHECK("k_block_norm_fwd");
   return MPNN_OK;
 }
 
 int64_t mpnn_block_norm_partial_floats(int64_t N, int32_t H, int32_t dtype) {
+  (void)dtype;   // the slabs are float whatever the rows are
   if (N < 0 || H < 1 || H > kNormMaxH) return -1;
-  const bool bf16 = dtype == MPNN_BF16;
-  const int v = bf16 ? 8 : 4;
-  int blocks = norm_bwd_blocks(N, norm_shape(H, false, bf16));
-  if (H % v == 0) {
-    const int b = norm_bwd_blocks(N, norm_shape(H, true, bf16));
+  int blocks = norm_bwd_blocks(N, norm_lanes(H, false));
+  if (H % 4 == 0) {
+    const int b = norm_bwd_blocks(N, norm_lanes(H, true));
     if (b > blocks) blocks = b;
   }
   return (int64_t)blocks * kNormSums * H;
@@ -518,16 +657,17 @@ int32_t mpnn_block_norm_bwd(const mpnn_block_norm* d, mpnn_stream_t stream) {
   if (n > 0 && d->N > 0 && !d->partial) return fail(MPNN_E_INVALID, "mpnn_block_norm_bwd: null pointer argument");
   a.partial = d->partial;
   const bool bf16 = d->dtype == MPNN_BF16;
-  const NormShape s = norm_shape(d->H, wide, bf16);
-  const int blocks = norm_bwd_blocks(d->N, s);
+  const int lpr = norm_lanes(d->H, wide);
+  const int blocks = norm_bwd_blocks(d->N, lpr);
   if (d->N > 0) {
-    const bool known = bf16 ? dispatch_norm<bf16_t>(a, s, true, blocks, stream) : dispatch_norm<float>(a, s, true, blocks, stream);
+    const bool known = bf16 ? dispatch_norm<bf16_t>(a, wide, lpr, true, blocks, stream)
+                            : dispatch_norm<float>(a, wide, lpr, true, blocks, stream);
     if (!known) return fail(MPNN_E_INVALID, "mpnn_block_norm_bwd: no kernel for H=%d", d->H);
     MPNN_LAUNCH_CHECK("k_block_norm_bwd");
   }
   if (n > 0) {
     f.partial = d->partial; f.n_sums = n; f.H = d->H; f.blocks = d->N > 0 ? blocks : 0;
-    const int grid = (n * d->H + 63) / 64;
+    const int grid = (n * d->H + 15) / 16;
     if (bf16) k_block_norm_sums<bf16_t><<<grid, kBlock, 0, stream>>>(f);
     else k_block_norm_sums<float><<<grid, kBlock, 0, stream>>>(f);
     MPNN_LAUNCH_CHECK("k_block_norm_sums");
