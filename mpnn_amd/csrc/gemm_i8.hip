@@ -4,7 +4,15 @@
 //
 // the forward of a Linear call (models/layers.py:104,140, models/mpnn.py:101) of a trained model, with one scale per
 // row of x and one per output channel.  The sum is exact (32-bit integers: 127 * 127 * K stays below 2^31 for
-// K <= 8192), the scales are applied in float32 and the result is rounded once to the output type.
+// K <= 8192), the scales are applied in float32 and the result is rounded once to the output type, in the same steps
+// by every kernel here.  Weights are the first matrix operand, rows of x the second, so that a lane's results are
+// consecutive outputs of one row.  Bytes behind column K count as zeros on x's side, whatever the weights hold there.
+//
+// Three kernels:
+//   rows    K <= 512, weights resident in LDS: x is read once as it lies, taken to 8 bits in registers and multiplied
+//           from there.  Bound by memory.
+//   tiles   both sides staged through LDS in steps of 128 bytes by asynchronous copies.  Bound by the matrix cores.
+//   thin    few rows: a wave per 32 x 32 outputs, operands from memory as they lie.  Bound by latency.
 #include "common.h"
 #include "rowio.h"
 
@@ -17,87 +25,483 @@ typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 constexpr int kI8MaxK = 8192;
 
 struct I8Args {
-  const int8_t* x; int64_t ldx;
-  const float* xs;
+  const void* x; int64_t ldx;      // 8-bit rows, or float rows (rows kernel)
+  const float* xs;                 // of 8-bit rows
   const int8_t* w; int64_t ldw;
   const float* ws;
   const void* bias;
   void* y; int64_t ldy;
   int64_t N;
-  int K, M, relu;
+  int K, M, relu, wide_out;        // wide_out: 8 consecutive outputs can leave as 16-byte vectors
 };
 
-template <typename T>
-__device__ __forceinline__ void store_quad(T* p, const float (&v)[4], int left, bool wide) {
-  if (wide && left >= 4) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    else
-      *reinterpret_cast<uint2*>(p) = make_uint2((uint32_t)f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
-                                                (uint32_t)f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
+__device__ __forceinline__ float finish(int32_t acc, float scale, float bias, int relu) {
+  const float v = fmaf((float)acc, scale, bias);
+  return relu && v <= 0.f ? 0.f : v;      // a NaN stays
+}
+
+// 16 bytes of which the first `left` are columns; the others count as zeros.
+__device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int left) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int l = left - 4 * j;
+    v[j] = l >= 4 ? v[j] : (l <= 0 ? 0 : (int32_t)((uint32_t)v[j] & ((1u << (8 * l)) - 1u)));
+  }
+  return v;
+}
+
+// V consecutive outputs of a row.
+template <typename Y, int V>
+__device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int left, bool wide) {
+  if (wide && left >= V) {
+    if constexpr (sizeof(Y) == 4) {
+#pragma unroll
+      for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+      uint32_t w[V / 2];
+#pragma unroll
+      for (int j = 0; j < V; j += 2) w[j / 2] = (uint32_t)f32_to_bf16(v[j]) | ((uint32_t)f32_to_bf16(v[j + 1]) << 16);
+      if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      else
+#pragma unroll
+        for (int j = 0; j < V / 2; j += 4) *reinterpret_cast<uint4*>(p + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < left) p[j] = f32_to_scalar<T>(v[j]);
+    for (int j = 0; j < V; ++j)
+      if (j < left) p[j] = f32_to_scalar<Y>(v[j]);
   }
 }
 
-// A wave owns 32 rows x 128 output columns (four 32 x 32 tiles, the weights as the first operand so that a lane holds
-// four consecutive outputs of one row); operands come from memory as they lie.
-template <typename T>
-__global__ void __launch_bounds__(kBlock) k_linear_i8(I8Args a, bool wide) {
+// ------------------------------------------------------------------------------------------------------------- rows
+// A wave owns 16 rows at a time.  Lane (row i = lane % 16, group g = lane / 16) holds 16 values of every step of 64
+// columns.  Which 16 is free as long as both operands agree, so they are the ones that make the loads whole: in float32
+// columns 16 p + 4 g .. + 3 (a row's four groups read 64 consecutive bytes per load), in bfloat16 32 p + 8 g .. + 7, in
+// 8 bits 16 g .. + 15; the weights are brought into that order on their way to LDS, once per block.
+// Output column m of a pair of 16-column tiles t lies in row 16 t + i of the pair with m = 8 (i / 4) + 4 t + i % 4: a
+// lane ends with 8 consecutive outputs.
+constexpr int kI8RowsThreads = 512;
+constexpr int kI8RowsLds = 144 * 1024;
+
+template <typename X> struct XRaw;
+template <> struct XRaw<float> { float v[16]; };
+template <> struct XRaw<bf16_t> { uint32_t v[8]; };
+template <> struct XRaw<int8_t> { i32x4 v; };
+
+template <typename X, bool WIDE>
+__device__ __forceinline__ void load_x(const X* p, int s, int g, int K, XRaw<X>& r) {
+  if constexpr (sizeof(X) == 4) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int k = 64 * s + 16 * q + 4 * g;
+      if constexpr (WIDE) {   // K is a multiple of 4
+        const float4 t = *reinterpret_cast<const float4*>(p + (k < K ? k : 0));
+        r.v[4 * q] = t.x; r.v[4 * q + 1] = t.y; r.v[4 * q + 2] = t.z; r.v[4 * q + 3] = t.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[4 * q + e] = p[k + e < K ? k + e : 0];
+      }
+    }
+  } else if constexpr (sizeof(X) == 2) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int k = 64 * s + 32 * q + 8 * g;
+      if constexpr (WIDE) {   // K is a multiple of 8
+        const uint4 t = *reinterpret_cast<const uint4*>(p + (k < K ? k : 0));
+        r.v[4 * q] = t.x; r.v[4 * q + 1] = t.y; r.v[4 * q + 2] = t.z; r.v[4 * q + 3] = t.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          r.v[4 * q + e / 2] = (uint32_t)p[k + e < K ? k + e : 0] | ((uint32_t)p[k + e + 1 < K ? k + e + 1 : 0] << 16);
+      }
+    }
+  } else {
+    const int k = 64 * s + 16 * g;
+    r.v = *reinterpret_cast<const i32x4*>(p + (k < K ? k : 0));   // rows are readable up to K rounded up to 16
+  }
+}
+
+// The step's 16 values in operand order, zeros for columns from K on.
+template <typename X>
+__device__ __forceinline__ void values_of(const XRaw<X>& r, int s, int g, int K, float (&v)[16]) {
+  if constexpr (sizeof(X) == 4) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = r.v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[2 * e] = __uint_as_float(r.v[e] << 16);
+      v[2 * e + 1] = __uint_as_float(r.v[e] & 0xffff0000u);
+    }
+  }
+  if (64 * s + 64 > K)   // uniform
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int k = sizeof(X) == 4 ? 64 * s + 16 * (e / 4) + 4 * g + e % 4 : 64 * s + 32 * (e / 8) + 8 * g + e % 8;
+      v[e] = k < K ? v[e] : 0.f;
+    }
+}
+
+// Waves per SIMD that the registers are held to: 16 waves per CU, 8 where a tile's raw rows take more than half of them.
+template <typename X>
+constexpr int rows_waves(int ks) { return ks == 8 || ks * sizeof(X) * 4 > 48 ? 2 : 4; }
+
+template <typename X, typename Y, int KS, bool WIDE>
+__global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8_rows(I8Args a, int slice) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int PITCH = KS * 64 + 16;   // 16 bytes more: eight consecutive rows start in different banks
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  const int m_begin = (int)blockIdx.y * slice;
+  const int m_count = a.M - m_begin < slice ? a.M - m_begin : slice;
+  const int m_pad = (m_count + 31) & ~31;
+  const int Kp = (a.K + 15) & ~15, steps = (a.K + 63) >> 6;
+  float* const s_ws = reinterpret_cast<float*>(lds + m_pad * PITCH);
+  float* const s_bias = s_ws + m_pad;
+  const X* const x = static_cast<const X*>(a.x);
+
+  const int64_t tiles = (a.N + 15) >> 4, step = (int64_t)gridDim.x * (kI8RowsThreads / 64);
+  int64_t tile = (int64_t)blockIdx.x * (kI8RowsThreads / 64) + wave;
+  XRaw<X> raw[KS];
+  float held = 0.f;
+  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+    const int64_t row = 16 * t + i < a.N ? 16 * t + i : a.N - 1;
+    if constexpr (sizeof(X) == 1) held = a.xs[row];
+    int from = g;
+    asm volatile("" : "+v"(from));   // the column offsets are formed anew per tile: kept, they would not fit the registers
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      if (s < steps) load_x<X, WIDE>(x + row * a.ldx, s, from, a.K, raw[s]);
+  };
+  if (tile < tiles) fetch(tile);
+
+  for (int idx = threadIdx.x; idx < m_pad * (KS * 4); idx += kI8RowsThreads) {
+    const int pos = idx / (KS * 4), c = idx - pos * (KS * 4);
+    if (16 * c >= Kp) continue;         // never multiplied by anything but zeros
+    const int r = pos & 15;
+    const int m = m_begin + (pos & ~31) + 8 * (r >> 2) + 4 * ((pos >> 4) & 1) + (r & 3);
+    const i32x4 v = *reinterpret_cast<const i32x4*>(a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw + 16 * c);
+    char* d = lds + pos * PITCH + (c >> 2) * 64;
+    const int cc = c & 3;
+    if constexpr (sizeof(X) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<int32_t*>(d + j * 16 + cc * 4) = v[j];
+    } else if constexpr (sizeof(X) == 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int u = 2 * cc + h;
+        *reinterpret_cast<int2*>(d + (2 * (u & 3) + (u >> 2)) * 8) = make_int2(v[2 * h], v[2 * h + 1]);
+      }
+    } else {
+      *reinterpret_cast<i32x4*>(d + cc * 16) = v;
+    }
+  }
+  for (int j = threadIdx.x; j < m_pad; j += kI8RowsThreads) {
+    const int m = m_begin + j < a.M ? m_begin + j : a.M - 1;
+    s_ws[j] = a.ws[m];
+    s_bias[j] = a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[m]) : 0.f;
+  }
+  __syncthreads();
+
+  for (; tile < tiles; tile += step) {
+    i32x4 q[KS];
+    float xs;
+    if constexpr (sizeof(X) == 1) {
+      xs = held;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] = 64 * s + 64 > a.K ? keep_bytes(raw[s].v, a.K - 64 * s - 16 * g) : raw[s].v;
+    } else {
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        if (s < steps) {
+          float v[16];
+          values_of<X>(raw[s], s, g, a.K, v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+            top = m > top ? m : top;
+          }
+        }
+      {   // the row's other three groups
+        uint32_t o = __shfl_xor(top, 16, 64);
+        top = o > top ? o : top;
+        o = __shfl_xor(top, 32, 64);
+        top = o > top ? o : top;
+      }
+      const bool finite = top < 0x7f800000u, zero = __uint_as_float(top) < 0x1p-100f;
+      const float inv = (zero || !finite) ? 0.f : 127.f / __uint_as_float(top);
+      xs = !finite ? __builtin_nanf("") : (zero ? 0.f : __uint_as_float(top) / 127.f);
+      const uint32_t keep = finite ? ~0u : 0u;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        if (s < steps) {
+          float v[16];
+          values_of<X>(raw[s], s, g, a.K, v);
+          uint32_t b[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) b[e] = __float_as_uint(fmaf(v[e], inv, 12582912.f));   // rows8.hip: whole numbers in the last place
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = __builtin_amdgcn_perm(b[4 * j + 1], b[4 * j], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(b[4 * j + 3], b[4 * j + 2], 0x04000c0cu);
+            q[s][j] = (int32_t)((lo | hi) & keep);
+          }
+        }
+    }
+    const int64_t row = 16 * tile + i;
+    if (tile + step < tiles) fetch(tile + step);
+    Y* const y = static_cast<Y*>(a.y) + row * a.ldy + m_begin;
+    for (int b = 0; b < m_pad; b += 32) {
+      i32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      const char* w = lds + (b + i) * PITCH + g * 16;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        if (s < steps)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(w + t * 16 * PITCH + s * 64), q[s], acc[t], 0, 0, 0);
+      float v[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float4 ws = *reinterpret_cast<const float4*>(s_ws + b + 8 * g + 4 * t);
+        const float4 bs = *reinterpret_cast<const float4*>(s_bias + b + 8 * g + 4 * t);
+        v[4 * t] = finish(acc[t][0], xs * ws.x, bs.x, a.relu);
+        v[4 * t + 1] = finish(acc[t][1], xs * ws.y, bs.y, a.relu);
+        v[4 * t + 2] = finish(acc[t][2], xs * ws.z, bs.z, a.relu);
+        v[4 * t + 3] = finish(acc[t][3], xs * ws.w, bs.w, a.relu);
+      }
+      if (row < a.N) store_outputs<Y, 8>(y + b + 8 * g, v, m_count - b - 8 * g, a.wide_out);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- thin
+// A block owns 32 rows x 128 outputs, a wave 32 x 32 of them.
+template <typename Y>
+__global__ void __launch_bounds__(kBlock) k_linear_i8_thin(I8Args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i32 = lane & 31, half = lane >> 5;
-  const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * 32;
-  const int m0 = (int)blockIdx.y * 128;
-  if (n0 >= a.N) return;
+  const int64_t n0 = (int64_t)blockIdx.x * 32;
+  const int m0 = (int)blockIdx.y * 128 + 32 * wave;
+  if (m0 >= a.M) return;
   const int64_t row = n0 + i32 < a.N ? n0 + i32 : a.N - 1;
   const int Kp = (a.K + 15) & ~15;
-  const int8_t* xp = a.x + row * a.ldx;
-  const int8_t* wp[4];
+  const int8_t* xp = static_cast<const int8_t*>(a.x) + row * a.ldx;
+  const int8_t* wp = a.w + (int64_t)(m0 + i32 < a.M ? m0 + i32 : a.M - 1) * a.ldw;
+  i32x16 acc;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int m = m0 + 32 * t + i32;
-    wp[t] = a.w + (int64_t)(m < a.M ? m : 0) * a.ldw;
-  }
-  i32x16 acc[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[t][r] = 0;
+  for (int r = 0; r < 16; ++r) acc[r] = 0;
+#pragma unroll 8
   for (int k0 = 0; k0 < Kp; k0 += 32) {
     const int k = k0 + 16 * half;
     const int off = k < Kp ? k : 0;
-    i32x4 x = *reinterpret_cast<const i32x4*>(xp + off);
-    const int left = a.K - k;   // bytes of this lane that are columns; the others count as zeros
-    if (left < 16)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int l = left - 4 * j;
-        x[j] = l >= 4 ? x[j] : (l <= 0 ? 0 : (int32_t)((uint32_t)x[j] & ((1u << (8 * l)) - 1u)));
-      }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const i32x4*>(wp[t] + off), x, acc[t], 0, 0, 0);
+    const i32x4 x = keep_bytes(*reinterpret_cast<const i32x4*>(xp + off), a.K - k);
+    acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const i32x4*>(wp + off), x, acc, 0, 0, 0);
   }
   if (n0 + i32 >= a.N) return;
   const float xs = a.xs[row];
-  T* y = static_cast<T*>(a.y) + row * a.ldy;
+  Y* y = static_cast<Y*>(a.y) + row * a.ldy;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int q = 0; q < 4; ++q) {
+    const int m = m0 + 8 * q + 4 * half;
+    if (m >= a.M) continue;
+    float v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int m = m0 + 32 * t + 8 * q + 4 * half;
-      if (m >= a.M) continue;
-      float v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int mj = m + j < a.M ? m + j : a.M - 1;
-        v[j] = (float)acc[t][4 * q + j] * (xs * a.ws[mj]);
-        if (a.bias) v[j] += scalar_to_f32(static_cast<const T*>(a.bias)[mj]);
-        if (a.relu) v[j] = v[j] <= 0.f ? 0.f : v[j];   // a NaN stays
-      }
-      store_quad(y + m, v, a.M - m, wide);
+    for (int j = 0; j < 4; ++j) {
+      const int mj = m + j < a.M ? m + j : a.M - 1;
+      v[j] = finish(acc[4 * q + j], xs * a.ws[mj], a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[mj]) : 0.f, a.relu);
     }
+    store_outputs<Y, 4>(y + m, v, a.M - m, a.wide_out);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ tiles
+// A block of WN x WM waves owns WN * 32 TN rows x WM * 64 outputs; a wave TN x 2 tiles of 32 x 32.  Steps of 128 bytes
+// of K: rows lie in LDS 128 bytes apart, their eight 16-byte pieces in an order that depends on the row (piece c of row
+// r at c ^ (r % 8)), so that the 8 lanes of a read group reach 8 different bank groups; the copies go straight to LDS
+// in that order because a lane chooses where it reads, not where it writes.  The next step's copies run under this
+// step's products.
+// Output column m of a wave lies in row 32 t + i of its weight tiles with m = 32 ((i / 4) % 2) + 16 t + 4 (i / 8) + i % 4:
+// a lane ends with 32 consecutive outputs.
+__device__ const i32x4 kZeroPiece = {0, 0, 0, 0};
+
+template <int WN, int WM, int TN>
+constexpr int tiles_lds() { return 2 * (WN * TN * 32 + WM * 64) * 128; }
+
+template <typename Y, int WN, int WM, int TN>
+__global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, int n_tiles, int m_tiles) {
+  constexpr int BN = WN * TN * 32, BM = WM * 64, WAVES = WN * WM;
+  constexpr int STAGE = (BN + BM) * 128;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i32 = lane & 31, half = lane >> 5;
+  const int wn = wave / WM, wm = wave % WM;
+  // blocks go round the 8 XCDs: those of one XCD take all column tiles of a row tile one after the other, so that a
+  // row tile is fetched into one L2 only
+  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+  const int nt = (local / m_tiles) * 8 + xcd, mt = local % m_tiles;
+  if (nt >= n_tiles) return;
+  const int64_t n0 = (int64_t)nt * BN;
+  const int m0 = mt * BM;
+  const int Kp = (a.K + 15) & ~15, pieces = Kp >> 4;
+  const int8_t* const x = static_cast<const int8_t*>(a.x);
+
+  // copies: one instruction of a wave fills 8 rows (1 KiB); rows 0 .. BN - 1 are x's, the others weights
+  constexpr int COPIES = (BN + BM) / 8 / WAVES;
+  const int8_t* src[COPIES];
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) {
+    const int r = (c * WAVES + wave) * 8 + (lane >> 3);
+    if (r < BN) src[c] = x + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldx;
+    else {
+      const int p = r - BN, i = p & 31;
+      const int m = m0 + (p & ~63) + 32 * ((i >> 2) & 1) + 16 * ((p >> 5) & 1) + 4 * (i >> 3) + (i & 3);
+      src[c] = a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw;
+    }
+  }
+  const int piece = (lane & 7) ^ (lane >> 3);
+  auto stage = [&](int buf, int p0) __attribute__((always_inline)) {
+    const int at = p0 + piece;
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+      const int8_t* from = at < pieces ? src[c] + 16 * at : reinterpret_cast<const int8_t*>(&kZeroPiece);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                       (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (c * WAVES + wave) * 1024), 16, 0, 0);
+    }
+  };
+  i32x16 acc[TN][2];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][t][r] = 0;
+  stage(0, 0);
+  int buf = 0;
+  for (int p0 = 0; p0 < pieces; p0 += 8, buf ^= 1) {
+    __syncthreads();                       // this step's copies have landed, the other buffer is read no more
+    if (p0 + 8 < pieces) stage(buf ^ 1, p0 + 8);
+    const char* const xb = lds + buf * STAGE + (wn * TN * 32 + i32) * 128;
+    const char* const wb = lds + buf * STAGE + (BN + wm * 64 + i32) * 128;
+    const bool partial = (a.K & 15) && p0 + 8 >= pieces;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const int slot = ((2 * kk + half) ^ (lane & 7)) * 16;
+      i32x4 w[2], v[TN];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) w[t] = *reinterpret_cast<const i32x4*>(wb + t * 32 * 128 + slot);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) v[j] = *reinterpret_cast<const i32x4*>(xb + j * 32 * 128 + slot);
+      if (partial)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) v[j] = keep_bytes(v[j], a.K - 16 * (p0 + 2 * kk + half));
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[t], v[j], acc[j][t], 0, 0, 0);
+    }
+  }
+  const int mb = m0 + wm * 64 + 32 * half;
+  if (mb >= a.M) return;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int64_t row = n0 + (wn * TN + j) * 32 + i32;
+    if (row >= a.N) continue;
+    const float xs = a.xs[row];
+    Y* const y = static_cast<Y*>(a.y) + row * a.ldy + mb;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int m = mb + 16 * t + 8 * h + e;
+          const int mc = m < a.M ? m : a.M - 1;
+          v[e] = finish(acc[j][t][8 * h + e], xs * a.ws[mc], a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[mc]) : 0.f, a.relu);
+        }
+        store_outputs<Y, 8>(y + 16 * t + 8 * h, v, a.M - mb - 16 * t - 8 * h, a.wide_out);
+      }
+  }
+}
+
+// --------------------------------------------------------------------------------------------------------- dispatch
+enum class I8Kernel { kRows, kThin, kTiles };
+
+// Rows: the row in registers (K <= 512) and the weights in at most two slices of a CU's LDS (x is read once per slice),
+// or so few rows that reading them again does not count.  Thin: fewer rows than fill the smaller tile twice.
+I8Kernel i8_kernel(int64_t N, int K, int M) {
+  if (K <= 512) {
+    const int pitch = (K <= 64 ? 1 : K <= 128 ? 2 : K <= 256 ? 4 : 8) * 64 + 16 + 8;
+    if (N <= 1024 || (int64_t)((M + 31) / 32 * 32) * pitch <= 2 * kI8RowsLds) return I8Kernel::kRows;
+  }
+  return N <= 256 ? I8Kernel::kThin : I8Kernel::kTiles;
+}
+
+template <typename X, typename Y, int KS, bool WIDE>
+int32_t launch_rows(const I8Args& a, hipStream_t stream) {
+  const int m32 = (a.M + 31) / 32, per32 = 32 * (KS * 64 + 16 + 8);
+  const int64_t row_blocks = (a.N + 127) / 128;     // 8 waves of 16 rows
+  // weights: as few slices as fit, more of them when the rows alone would leave CUs without work
+  int slices = (m32 * per32 + kI8RowsLds - 1) / kI8RowsLds;
+  while (slices < m32 && row_blocks * slices < 256) ++slices;
+  int per = (m32 + slices - 1) / slices;
+  slices = (m32 + per - 1) / per;
+  const int bytes = per * per32;
+  int per_cu = 160 * 1024 / bytes;
+  const int by_regs = rows_waves<X>(KS) / 2;
+  if (per_cu > by_regs) per_cu = by_regs;
+  int64_t blocks = 256 * per_cu / slices;
+  if (blocks < 1) blocks = 1;
+  if (blocks > row_blocks) blocks = row_blocks;
+  if (bytes > 64 * 1024)
+    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_rows<X, Y, KS, WIDE>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  k_linear_i8_rows<X, Y, KS, WIDE><<<dim3((unsigned)blocks, slices), kI8RowsThreads, bytes, stream>>>(a, per * 32);
+  MPNN_LAUNCH_CHECK("k_linear_i8_rows");
+  return MPNN_OK;
+}
+
+template <typename X, typename Y, bool WIDE>
+int32_t rows_of(const I8Args& a, hipStream_t stream) {
+  if (a.K <= 64) return launch_rows<X, Y, 1, WIDE>(a, stream);
+  if (a.K <= 128) return launch_rows<X, Y, 2, WIDE>(a, stream);
+  if (a.K <= 256) return launch_rows<X, Y, 4, WIDE>(a, stream);
+  return launch_rows<X, Y, 8, WIDE>(a, stream);
+}
+
+template <typename Y, int WN, int WM, int TN>
+int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
+  constexpr int BN = WN * TN * 32, BM = WM * 64, bytes = tiles_lds<WN, WM, TN>();
+  const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
+  const int64_t grid = (nt + 7) / 8 * 8 * mt;
+  if (grid > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld M=%d", (long long)a.N, a.M);
+  if (bytes > 64 * 1024)
+    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_tiles<Y, WN, WM, TN>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  k_linear_i8_tiles<Y, WN, WM, TN><<<(unsigned)grid, WN * WM * 64, bytes, stream>>>(a, (int)nt, (int)mt);
+  MPNN_LAUNCH_CHECK("k_linear_i8_tiles");
+  return MPNN_OK;
+}
+
+template <typename Y>
+int32_t launch_i8(const I8Args& a, I8Kernel kernel, int x_dtype, bool wide_in, hipStream_t stream) {
+  if (kernel == I8Kernel::kRows) {
+    if (x_dtype == MPNN_I8) return rows_of<int8_t, Y, true>(a, stream);
+    if (x_dtype == MPNN_F32) return wide_in ? rows_of<float, Y, true>(a, stream) : rows_of<float, Y, false>(a, stream);
+    return wide_in ? rows_of<bf16_t, Y, true>(a, stream) : rows_of<bf16_t, Y, false>(a, stream);
+  }
+  if (kernel == I8Kernel::kThin) {
+    if ((a.M + 127) / 128 > 65535) return fail(MPNN_E_INVALID, "mpnn_linear_int8: M=%d", a.M);
+    const dim3 grid((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 127) / 128));
+    k_linear_i8_thin<Y><<<grid, kBlock, 0, stream>>>(a);
+    MPNN_LAUNCH_CHECK("k_linear_i8_thin");
+    return MPNN_OK;
+  }
+  // tiles of 256 x 256 if they fill the CUs, of 128 x 128 otherwise
+  if (((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, 2, 4, 4>(a, stream);
+  return launch_tiles<Y, 2, 2, 2>(a, stream);
 }
 
 }  // namespace
@@ -109,7 +513,7 @@ extern "C" {
 
 int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_t x_dtype) {
   if (N < 0 || K < 1 || K > kI8MaxK || M < 1) return -1;
-  if (x_dtype == MPNN_I8) return 0;
+  if (x_dtype == MPNN_I8 || i8_kernel(N, K, M) == I8Kernel::kRows) return 0;
   return N * ((K + 15) / 16 * 16) + align_up(N * 4, 16);
 }
 
@@ -118,29 +522,32 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
                          int32_t K, int32_t M, int32_t relu, void* workspace, mpnn_stream_t stream) {
   if ((x_dtype != MPNN_F32 && x_dtype != MPNN_BF16 && x_dtype != MPNN_I8) || (y_dtype != MPNN_F32 && y_dtype != MPNN_BF16))
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: dtypes %d, %d", x_dtype, y_dtype);
-  if (N < 0 || K < 1 || K > kI8MaxK || M < 1) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld K=%d M=%d (K up to %d)", (long long)N, K, M, kI8MaxK);
+  if (N < 0 || K < 1 || K > kI8MaxK || M < 1 || M > (1 << 24))
+    return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld K=%d M=%d (K up to %d)", (long long)N, K, M, kI8MaxK);
   const int Kp = (K + 15) / 16 * 16;
   if (ldx < (x_dtype == MPNN_I8 ? Kp : K) || ldw < Kp || ldy < M) return fail(MPNN_E_INVALID, "mpnn_linear_int8: leading dimension too small");
   if (N == 0) return MPNN_OK;
-  if (!X || !W || !w_scale || !Y || (x_dtype == MPNN_I8 ? !x_scale : !workspace)) return fail(MPNN_E_INVALID, "mpnn_linear_int8: null pointer argument");
+  const I8Kernel kernel = i8_kernel(N, K, M);
+  const bool take = x_dtype != MPNN_I8 && kernel != I8Kernel::kRows;     // to 8 bits in a pass of its own
+  if (!X || !W || !w_scale || !Y || (x_dtype == MPNN_I8 && !x_scale) || (take && !workspace))
+    return fail(MPNN_E_INVALID, "mpnn_linear_int8: null pointer argument");
   if (((uintptr_t)W & 15) || (ldw & 15) || (x_dtype == MPNN_I8 && (((uintptr_t)X & 15) || (ldx & 15))) || ((uintptr_t)workspace & 15))
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: 8-bit rows and the workspace must be 16-byte aligned");
-  I8Args a{static_cast<const int8_t*>(X), ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu};
-  if (x_dtype != MPNN_I8) {
+  if ((N + 31) / 32 > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld", (long long)N);
+  const int vec = y_dtype == MPNN_BF16 ? 8 : 4;
+  const int wide_out = ((uintptr_t)Y & 15) == 0 && ldy % vec == 0;
+  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out};
+  if (take) {
     int8_t* q = static_cast<int8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + N * Kp);
     const int32_t rc = mpnn_quantize_rows(X, ldx, x_dtype, N, K, q, Kp, s, stream);
     if (rc != MPNN_OK) return rc;
     a.x = q; a.ldx = Kp; a.xs = s;
   }
-  if ((N + 127) / 128 > INT32_MAX || (M + 127) / 128 > 65535) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld M=%d", (long long)N, M);
-  const dim3 grid((unsigned)((N + 127) / 128), (unsigned)((M + 127) / 128));
-  const int quad = y_dtype == MPNN_BF16 ? 8 : 16;
-  const bool wide = ((uintptr_t)Y % quad) == 0 && ldy % 4 == 0;
-  if (y_dtype == MPNN_BF16) k_linear_i8<bf16_t><<<grid, kBlock, 0, stream>>>(a, wide);
-  else k_linear_i8<float><<<grid, kBlock, 0, stream>>>(a, wide);
-  MPNN_LAUNCH_CHECK("k_linear_i8");
-  return MPNN_OK;
+  const int xvec = x_dtype == MPNN_BF16 ? 8 : 4;
+  const bool wide_in = K % xvec == 0 && ldx % xvec == 0 && ((uintptr_t)X & 15) == 0;
+  return y_dtype == MPNN_BF16 ? launch_i8<bf16_t>(a, kernel, x_dtype, wide_in, stream)
+                              : launch_i8<float>(a, kernel, x_dtype, wide_in, stream);
 }
 
 }  // extern "C"

@@ -141,19 +141,49 @@ def test_linear_int8(n, k, m):
 
 
 @pytest.mark.gpu
-def test_linear_int8_bytes_behind_the_rows_do_not_count():
+@pytest.mark.parametrize("n,k,m", [(4133, 520, 4091), (4096, 1040, 4160), (3000, 513, 70), (777, 1111, 777), (300, 4099, 130),
+                                   (20000, 512, 300), (33, 512, 3000), (1100, 300, 1100), (50000, 500, 192), (70000, 64, 64)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_linear_int8_many_rows(n, k, m, out):
+    """Every kernel at sizes with whole and ragged tiles; 64-bit products on the device."""
+    from mpnn_amd import linear_int8, quantize_rows
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(n, k, generator=gen, device="cuda")
+    w = torch.randn(m, k, generator=gen, device="cuda")
+    b = torch.randn(m, generator=gen, device="cuda").to(out)
+    xr, wr = quantize_rows(x), quantize_rows(w)
+    want = (xr.values.double() @ wr.values.double().t()) * (xr.scale.double().unsqueeze(1) * wr.scale.double())
+    bound = 3 * U * want.abs()
+    want = want + b.double()
+    bound += U * want.abs()
+    bound += torch.finfo(out).eps / 2 * (want.abs() + bound)
+    for rows in (x, xr):
+        got = linear_int8(rows, wr, bias=b, dtype=out)
+        assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,m", [(50, 21, 30), (50, 530, 30), (300, 530, 30)])
+def test_linear_int8_bytes_behind_the_rows_do_not_count_anywhere(n, k, m):
     from mpnn_amd import Rows8, linear_int8, quantize_rows
-    x, w = randn(50, 21, seed=1), randn(30, 21, seed=2)
+    x, w = randn(n, k, seed=1), randn(m, k, seed=2)
     want = linear_int8(x.cuda(), quantize_rows(w.cuda()))
     dirty = []
     for t in (x, w):
         r = quantize_rows(t.cuda())
-        store = torch.full((t.size(0), 48), 77, dtype=torch.int8, device="cuda")
-        store[:, :21] = r.values
-        rows = Rows8(store[:, :21], r.scale)
+        store = torch.full((t.size(0), 560), 77, dtype=torch.int8, device="cuda")
+        store[:, :k] = r.values
+        rows = Rows8(store[:, :k], r.scale)
         assert rows.values.data_ptr() == store.data_ptr()
         dirty.append(rows)
     assert torch.equal(linear_int8(*dirty), want)
+
+
+@pytest.mark.gpu
+def test_linear_int8_layouts_that_cannot_be_read_in_place():
+    from mpnn_amd import Rows8, linear_int8, quantize_rows
+    x, w = randn(50, 21, seed=1), randn(30, 21, seed=2)
+    want = linear_int8(x.cuda(), quantize_rows(w.cuda()))
     # layouts that cannot be read in place are copied: odd pitch, columns of a wider matrix, a last row that ends early
     tight = quantize_rows(w.cuda()).values.contiguous()
     assert tight.stride(0) == 21
