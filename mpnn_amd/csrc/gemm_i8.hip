@@ -22,6 +22,9 @@ namespace {
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
+#ifndef I8BIG
+#define I8BIG 2, 4, 4, 8
+#endif
 constexpr int kI8MaxK = 8192;
 
 struct I8Args {
@@ -32,7 +35,9 @@ struct I8Args {
   const void* bias;
   void* y; int64_t ldy;
   int64_t N;
-  int K, M, relu, wide_out;        // wide_out: 8 consecutive outputs can leave as 16-byte vectors
+  int K, M, relu;
+  int wide_out;                    // 8 consecutive outputs can leave as 16-byte vectors
+  int wide_vectors;                // weight scales and biases can be read four at a time
 };
 
 __device__ __forceinline__ float finish(int32_t acc, float scale, float bias, int relu) {
@@ -78,8 +83,9 @@ __device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int lef
 // columns.  Which 16 is free as long as both operands agree, so they are the ones that make the loads whole: in float32
 // columns 16 p + 4 g .. + 3 (a row's four groups read 64 consecutive bytes per load), in bfloat16 32 p + 8 g .. + 7, in
 // 8 bits 16 g .. + 15; the weights are brought into that order on their way to LDS, once per block.
-// Output column m of a pair of 16-column tiles t lies in row 16 t + i of the pair with m = 8 (i / 4) + 4 t + i % 4: a
-// lane ends with 8 consecutive outputs.
+// A result tile leaves lane (row, g) with the tile's weight rows 4 g .. 4 g + 3.  float32 results leave as they are, 16
+// bytes per lane and 64 consecutive ones per row and store; for bfloat16 the weight rows of a pair of tiles t are laid so
+// that a lane ends with 8 consecutive outputs: column 8 (i / 4) + 4 t + i % 4 of the pair in row 16 t + i.
 constexpr int kI8RowsThreads = 512;
 constexpr int kI8RowsLds = 144 * 1024;
 
@@ -179,7 +185,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
     const int pos = idx / (KS * 4), c = idx - pos * (KS * 4);
     if (16 * c >= Kp) continue;         // never multiplied by anything but zeros
     const int r = pos & 15;
-    const int m = m_begin + (pos & ~31) + 8 * (r >> 2) + 4 * ((pos >> 4) & 1) + (r & 3);
+    const int m = m_begin + (sizeof(Y) == 4 ? pos : (pos & ~31) + 8 * (r >> 2) + 4 * ((pos >> 4) & 1) + (r & 3));
     const i32x4 v = *reinterpret_cast<const i32x4*>(a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw + 16 * c);
     char* d = lds + pos * PITCH + (c >> 2) * 64;
     const int cc = c & 3;
@@ -261,17 +267,26 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
 #pragma unroll
           for (int t = 0; t < 2; ++t)
             acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(w + t * 16 * PITCH + s * 64), q[s], acc[t], 0, 0, 0);
-      float v[8];
+      float v[2][4];
+      auto first_of = [&](int t) { return b + (sizeof(Y) == 4 ? 16 * t + 4 * g : 8 * g + 4 * t); };
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const float4 ws = *reinterpret_cast<const float4*>(s_ws + b + 8 * g + 4 * t);
-        const float4 bs = *reinterpret_cast<const float4*>(s_bias + b + 8 * g + 4 * t);
-        v[4 * t] = finish(acc[t][0], xs * ws.x, bs.x, a.relu);
-        v[4 * t + 1] = finish(acc[t][1], xs * ws.y, bs.y, a.relu);
-        v[4 * t + 2] = finish(acc[t][2], xs * ws.z, bs.z, a.relu);
-        v[4 * t + 3] = finish(acc[t][3], xs * ws.w, bs.w, a.relu);
+        const float4 ws = *reinterpret_cast<const float4*>(s_ws + first_of(t));
+        const float4 bs = *reinterpret_cast<const float4*>(s_bias + first_of(t));
+        v[t][0] = finish(acc[t][0], xs * ws.x, bs.x, a.relu);
+        v[t][1] = finish(acc[t][1], xs * ws.y, bs.y, a.relu);
+        v[t][2] = finish(acc[t][2], xs * ws.z, bs.z, a.relu);
+        v[t][3] = finish(acc[t][3], xs * ws.w, bs.w, a.relu);
       }
-      if (row < a.N) store_outputs<Y, 8>(y + b + 8 * g, v, m_count - b - 8 * g, a.wide_out);
+      if (row < a.N) {
+        if constexpr (sizeof(Y) == 4) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) store_outputs<Y, 4>(y + first_of(t), v[t], m_count - first_of(t), a.wide_out);
+        } else {
+          const float w[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+          store_outputs<Y, 8>(y + b + 8 * g, w, m_count - b - 8 * g, a.wide_out);
+        }
+      }
     }
   }
 }
@@ -317,50 +332,60 @@ __global__ void __launch_bounds__(kBlock) k_linear_i8_thin(I8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ tiles
-// A block of WN x WM waves owns WN * 32 TN rows x WM * 64 outputs; a wave TN x 2 tiles of 32 x 32.  Steps of 128 bytes
-// of K: rows lie in LDS 128 bytes apart, their eight 16-byte pieces in an order that depends on the row (piece c of row
-// r at c ^ (r % 8)), so that the 8 lanes of a read group reach 8 different bank groups; the copies go straight to LDS
-// in that order because a lane chooses where it reads, not where it writes.  The next step's copies run under this
-// step's products.
+// A block of WN x WM waves owns WN * 32 TN rows x WM * 64 outputs; a wave TN x 2 tiles of 32 x 32.  Steps of PC 16-byte
+// pieces of K (8 or 4): rows lie in LDS PC pieces apart, their pieces in an order that depends on the row, so that the 8
+// lanes of a read group reach 8 different bank groups; the copies go straight to LDS in that order because a lane
+// chooses where it reads, not where it writes.  The next step's copies run under this step's products.
 // Output column m of a wave lies in row 32 t + i of its weight tiles with m = 32 ((i / 4) % 2) + 16 t + 4 (i / 8) + i % 4:
 // a lane ends with 32 consecutive outputs.
 __device__ const i32x4 kZeroPiece = {0, 0, 0, 0};
 
-template <int WN, int WM, int TN>
-constexpr int tiles_lds() { return 2 * (WN * TN * 32 + WM * 64) * 128; }
+template <int WN, int WM, int TN, int PC>
+constexpr int tiles_lds() { return 2 * (WN * TN * 32 + WM * 64) * 16 * PC; }
 
-template <typename Y, int WN, int WM, int TN>
+// Piece c of row r lies at this place of the row.
+template <int PC>
+__device__ __forceinline__ int piece_at(int r, int c) { return PC == 8 ? c ^ (r & 7) : c ^ ((r >> 1) & 3); }
+
+template <typename Y, int WN, int WM, int TN, int PC>
 __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, int n_tiles, int m_tiles) {
   constexpr int BN = WN * TN * 32, BM = WM * 64, WAVES = WN * WM;
-  constexpr int STAGE = (BN + BM) * 128;
+  constexpr int ROW = 16 * PC, STAGE = (BN + BM) * ROW;
+  // results leave through the buffer that was read last: per wave 32 rows x 64 outputs
+  constexpr int VEC = 16 / sizeof(Y), CHUNKS = 64 / VEC, PATCH = 32 * 64 * sizeof(Y);
+  static_assert(WAVES * PATCH <= STAGE, "result patches fit a buffer");
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i32 = lane & 31, half = lane >> 5;
   const int wn = wave / WM, wm = wave % WM;
-  // blocks go round the 8 XCDs: those of one XCD take all column tiles of a row tile one after the other, so that a
-  // row tile is fetched into one L2 only
-  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-  const int nt = (local / m_tiles) * 8 + xcd, mt = local % m_tiles;
-  if (nt >= n_tiles) return;
-  const int64_t n0 = (int64_t)nt * BN;
-  const int m0 = mt * BM;
+  // Blocks stay and go round the tiles, those of one XCD (block index mod 8) through all column tiles of a row tile one
+  // after the other, so that a row tile is fetched into one L2 only.  A tile's last step already copies the next tile's
+  // first, and its results leave while that is on its way.
+  const int xcd = blockIdx.x & 7, turn = gridDim.x >> 3;
   const int Kp = (a.K + 15) & ~15, pieces = Kp >> 4;
-  const int8_t* const x = static_cast<const int8_t*>(a.x);
 
-  // copies: one instruction of a wave fills 8 rows (1 KiB); rows 0 .. BN - 1 are x's, the others weights
-  constexpr int COPIES = (BN + BM) / 8 / WAVES;
+  // copies: one instruction of a wave fills 64 / PC rows (1 KiB); rows 0 .. BN - 1 are x's, the others weights
+  constexpr int COPIES = (BN + BM) * PC / 64 / WAVES;
   const int8_t* src[COPIES];
+  auto take = [&](int t) __attribute__((always_inline)) {   // false: no such tile
+    const int nt = (t / m_tiles) * 8 + xcd;
+    if (nt >= n_tiles) return false;
+    const int64_t n0 = (int64_t)nt * BN;
+    const int m0 = t % m_tiles * BM;
 #pragma unroll
-  for (int c = 0; c < COPIES; ++c) {
-    const int r = (c * WAVES + wave) * 8 + (lane >> 3);
-    if (r < BN) src[c] = x + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldx;
-    else {
-      const int p = r - BN, i = p & 31;
-      const int m = m0 + (p & ~63) + 32 * ((i >> 2) & 1) + 16 * ((p >> 5) & 1) + 4 * (i >> 3) + (i & 3);
-      src[c] = a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw;
+    for (int c = 0; c < COPIES; ++c) {
+      const int r = (c * WAVES + wave) * (64 / PC) + lane / PC;
+      if (r < BN) {
+        src[c] = static_cast<const int8_t*>(a.x) + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldx;
+      } else {
+        const int p = r - BN, i = p & 31;
+        const int m = m0 + (p & ~63) + 32 * ((i >> 2) & 1) + 16 * ((p >> 5) & 1) + 4 * (i >> 3) + (i & 3);
+        src[c] = a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw;
+      }
     }
-  }
-  const int piece = (lane & 7) ^ (lane >> 3);
+    return true;
+  };
+  const int piece = piece_at<PC>(lane / PC, lane % PC);   // (the copy's first row is a multiple of 8)
   auto stage = [&](int buf, int p0) __attribute__((always_inline)) {
     const int at = p0 + piece;
 #pragma unroll
@@ -370,59 +395,106 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
                                        (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (c * WAVES + wave) * 1024), 16, 0, 0);
     }
   };
-  i32x16 acc[TN][2];
+
+  int tile = blockIdx.x >> 3, buf = 0;
+  bool more = take(tile);
+  if (more) stage(0, 0);
+  while (more) {
+    const int64_t n0 = (int64_t)((tile / m_tiles) * 8 + xcd) * BN;
+    const int m0 = tile % m_tiles * BM;
+    tile += turn;
+    i32x16 acc[TN][2];
 #pragma unroll
-  for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[j][t][r] = 0;
-  stage(0, 0);
-  int buf = 0;
-  for (int p0 = 0; p0 < pieces; p0 += 8, buf ^= 1) {
-    __syncthreads();                       // this step's copies have landed, the other buffer is read no more
-    if (p0 + 8 < pieces) stage(buf ^ 1, p0 + 8);
-    const char* const xb = lds + buf * STAGE + (wn * TN * 32 + i32) * 128;
-    const char* const wb = lds + buf * STAGE + (BN + wm * 64 + i32) * 128;
-    const bool partial = (a.K & 15) && p0 + 8 >= pieces;
+        for (int r = 0; r < 16; ++r) acc[j][t][r] = 0;
+    for (int p0 = 0; p0 < pieces; p0 += PC, buf ^= 1) {
+      __syncthreads();                     // this step's copies have landed, the other buffer is read no more
+      if (p0 + PC < pieces) stage(buf ^ 1, p0 + PC);
+      else if ((more = take(tile))) stage(buf ^ 1, 0);
+      const char* const xb = lds + buf * STAGE + (wn * TN * 32 + i32) * ROW;
+      const char* const wb = lds + buf * STAGE + (BN + wm * 64 + i32) * ROW;
+      const bool partial = (a.K & 15) && p0 + PC >= pieces;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const int slot = ((2 * kk + half) ^ (lane & 7)) * 16;
-      i32x4 w[2], v[TN];
+      for (int kk = 0; kk < PC / 2; ++kk) {
+        const int slot = piece_at<PC>(lane, 2 * kk + half) * 16;
+        i32x4 w[2], v[TN];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) w[t] = *reinterpret_cast<const i32x4*>(wb + t * 32 * 128 + slot);
+        for (int t = 0; t < 2; ++t) w[t] = *reinterpret_cast<const i32x4*>(wb + t * 32 * ROW + slot);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) v[j] = *reinterpret_cast<const i32x4*>(xb + j * 32 * 128 + slot);
-      if (partial)
+        for (int j = 0; j < TN; ++j) v[j] = *reinterpret_cast<const i32x4*>(xb + j * 32 * ROW + slot);
+        if (partial)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) v[j] = keep_bytes(v[j], a.K - 16 * (p0 + 2 * kk + half));
+          for (int j = 0; j < TN; ++j) v[j] = keep_bytes(v[j], a.K - 16 * (p0 + 2 * kk + half));
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[t], v[j], acc[j][t], 0, 0, 0);
-    }
-  }
-  const int mb = m0 + wm * 64 + 32 * half;
-  if (mb >= a.M) return;
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int64_t row = n0 + (wn * TN + j) * 32 + i32;
-    if (row >= a.N) continue;
-    const float xs = a.xs[row];
-    Y* const y = static_cast<Y*>(a.y) + row * a.ldy + mb;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int m = mb + 16 * t + 8 * h + e;
-          const int mc = m < a.M ? m : a.M - 1;
-          v[e] = finish(acc[j][t][8 * h + e], xs * a.ws[mc], a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[mc]) : 0.f, a.relu);
-        }
-        store_outputs<Y, 8>(y + 16 * t + 8 * h, v, a.M - mb - 16 * t - 8 * h, a.wide_out);
+          for (int t = 0; t < 2; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[t], v[j], acc[j][t], 0, 0, 0);
       }
+    }
+    // scales and biases of the lane's 32 outputs, the same for every row
+    const int mw = m0 + wm * 64, mb = mw + 32 * half;
+    float ws[32], bs[32];
+    if (mw + 64 <= a.M && a.wide_vectors) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(a.ws + mb + e);
+        ws[e] = t.x; ws[e + 1] = t.y; ws[e + 2] = t.z; ws[e + 3] = t.w;
+        float u[4] = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias) EdgeIO<Y, 4>::load(static_cast<const Y*>(a.bias) + mb + e, u);
+        bs[e] = u[0]; bs[e + 1] = u[1]; bs[e + 2] = u[2]; bs[e + 3] = u[3];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int m = mb + e < a.M ? mb + e : a.M - 1;
+        ws[e] = a.ws[m];
+        bs[e] = a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[m]) : 0.f;
+      }
+    }
+    __syncthreads();                       // every wave has read its operands: the buffer may take results
+    char* const patch = lds + (buf ^ 1) * STAGE + wave * PATCH;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int64_t r0 = n0 + (wn * TN + j) * 32;
+      const float xs = a.xs[r0 + i32 < a.N ? r0 + i32 : a.N - 1];
+      // 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread
+#pragma unroll
+      for (int c = 0; c < 32 / VEC; ++c) {
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int o = c * VEC + e;
+          v[e] = finish(acc[j][o >> 4][o & 15], xs * ws[o], bs[o], a.relu);
+        }
+        const int chunk = half * (32 / VEC) + c;
+        store_outputs<Y, VEC>(reinterpret_cast<Y*>(patch + i32 * (64 * (int)sizeof(Y)) + ((chunk ^ i32) & (CHUNKS - 1)) * 16), v, VEC, true);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int q = 0; q < 32 * CHUNKS / 64; ++q) {
+        const int r = q * (64 / CHUNKS) + lane / CHUNKS, chunk = lane % CHUNKS;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(patch + r * (64 * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
+        const int left = a.M - mw - chunk * VEC;
+        if (r0 + r >= a.N || left <= 0) continue;
+        Y* const y = static_cast<Y*>(a.y) + (r0 + r) * a.ldy + mw + chunk * VEC;
+        if (a.wide_out && left >= VEC) {
+          *reinterpret_cast<i32x4*>(y) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e < left) {
+              if constexpr (sizeof(Y) == 4) y[e] = __uint_as_float((uint32_t)v[e]);
+              else y[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
+            }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 }
 
@@ -471,16 +543,18 @@ int32_t rows_of(const I8Args& a, hipStream_t stream) {
   return launch_rows<X, Y, 8, WIDE>(a, stream);
 }
 
-template <typename Y, int WN, int WM, int TN>
+template <typename Y, int WN, int WM, int TN, int PC>
 int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
-  constexpr int BN = WN * TN * 32, BM = WM * 64, bytes = tiles_lds<WN, WM, TN>();
+  constexpr int BN = WN * TN * 32, BM = WM * 64, bytes = tiles_lds<WN, WM, TN, PC>();
   const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
-  const int64_t grid = (nt + 7) / 8 * 8 * mt;
-  if (grid > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld M=%d", (long long)a.N, a.M);
+  const int64_t all = (nt + 7) / 8 * 8 * mt;
+  const int64_t resident = 256 * (160 * 1024 / bytes);
+  const int64_t grid = all < resident ? all : resident;
+  if (all > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld M=%d", (long long)a.N, a.M);
   if (bytes > 64 * 1024)
-    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_tiles<Y, WN, WM, TN>),
+    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_tiles<Y, WN, WM, TN, PC>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  k_linear_i8_tiles<Y, WN, WM, TN><<<(unsigned)grid, WN * WM * 64, bytes, stream>>>(a, (int)nt, (int)mt);
+  k_linear_i8_tiles<Y, WN, WM, TN, PC><<<(unsigned)grid, WN * WM * 64, bytes, stream>>>(a, (int)nt, (int)mt);
   MPNN_LAUNCH_CHECK("k_linear_i8_tiles");
   return MPNN_OK;
 }
@@ -500,8 +574,8 @@ int32_t launch_i8(const I8Args& a, I8Kernel kernel, int x_dtype, bool wide_in, h
     return MPNN_OK;
   }
   // tiles of 256 x 256 if they fill the CUs, of 128 x 128 otherwise
-  if (((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, 2, 4, 4>(a, stream);
-  return launch_tiles<Y, 2, 2, 2>(a, stream);
+  if (((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, I8BIG>(a, stream);
+  return launch_tiles<Y, 2, 2, 2, 8>(a, stream);
 }
 
 }  // namespace
@@ -536,7 +610,8 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
   if ((N + 31) / 32 > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld", (long long)N);
   const int vec = y_dtype == MPNN_BF16 ? 8 : 4;
   const int wide_out = ((uintptr_t)Y & 15) == 0 && ldy % vec == 0;
-  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out};
+  const int wide_vectors = (((uintptr_t)w_scale | (uintptr_t)bias) & 15) == 0;
+  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out, wide_vectors};
   if (take) {
     int8_t* q = static_cast<int8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + N * Kp);
