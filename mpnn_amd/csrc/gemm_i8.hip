@@ -10,8 +10,11 @@
 //
 // Three kernels:
 //   rows    K <= 512, weights resident in LDS: x is read once as it lies, taken to 8 bits in registers and multiplied
-//           from there.  Bound by memory.
-//   tiles   both sides staged through LDS in steps of 128 bytes by asynchronous copies.  Bound by the matrix cores.
+//           from there.  Bound by memory: 4 M rows of 128 -> 256 in 0.64 ms (bfloat16, 4.8 TB/s) and 1.19 ms (float32, 5.2
+//           TB/s; a copy reaches 4.9), Flickr's 89,250 of 500 -> 192 in 56 us (float32, 4.4 TB/s).
+//   tiles   both sides staged through LDS in steps of 128 bytes by asynchronous copies.  65,536 x 1024 -> 2048 to
+//           bfloat16 in 216 us (1270 TOP/s), 4096^3 in 80 us (1710 TOP/s).  What bounds it: operand reads from LDS (192
+//           KiB per step of 128 and CU, three quarters of the matrix cores' time) and, for short K, the results.
 //   thin    few rows: a wave per 32 x 32 outputs, operands from memory as they lie.  Bound by latency.
 #include "common.h"
 #include "rowio.h"
@@ -22,10 +25,9 @@ namespace {
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
-#ifndef I8BIG
-#define I8BIG 2, 4, 4, 8
-#endif
 constexpr int kI8MaxK = 8192;
+
+constexpr int kI8MaxTileLd = 1 << 22;   // bytes from row to row: a tile's rows are reached by 32-bit offsets
 
 struct I8Args {
   const void* x; int64_t ldx;      // 8-bit rows, or float rows (rows kernel)
@@ -37,7 +39,6 @@ struct I8Args {
   int64_t N;
   int K, M, relu;
   int wide_out;                    // 8 consecutive outputs can leave as 16-byte vectors
-  int wide_vectors;                // weight scales and biases can be read four at a time
 };
 
 __device__ __forceinline__ float finish(int32_t acc, float scale, float bias, int relu) {
@@ -65,7 +66,7 @@ __device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int lef
     } else {
       uint32_t w[V / 2];
 #pragma unroll
-      for (int j = 0; j < V; j += 2) w[j / 2] = (uint32_t)f32_to_bf16(v[j]) | ((uint32_t)f32_to_bf16(v[j + 1]) << 16);
+      for (int j = 0; j < V; j += 2) w[j / 2] = pack_bf16(v[j], v[j + 1]);
       if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
       else
 #pragma unroll
@@ -78,16 +79,54 @@ __device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int lef
   }
 }
 
+// Results of a wave on their way to memory: ROWS rows x 64 outputs in LDS, from where whole row segments leave (128 bytes
+// in bfloat16, 256 in float32; stores of 64 bytes per row took 1.65 instead of 1.20 ms for 4 M rows of 256 in float32).
+// 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread.  Only
+// the wave that owns the patch touches it.
+template <typename Y, int ROWS>
+struct Patch {
+  static constexpr int VEC = 16 / sizeof(Y), CHUNKS = 64 / VEC, BYTES = ROWS * 64 * sizeof(Y);
+  char* base;
+  __device__ __forceinline__ void put(int row, int chunk, const float (&v)[VEC]) const {
+    store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (64 * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
+  }
+  // Rows r0 .. of the matrix, outputs m .. m + 63 of which those below `end` exist.
+  __device__ __forceinline__ void leave(const I8Args& a, int64_t r0, int m, int end) const {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < ROWS * CHUNKS / 64; ++q) {
+      const int r = q * (64 / CHUNKS) + lane / CHUNKS, chunk = lane % CHUNKS;
+      const i32x4 v = *reinterpret_cast<const i32x4*>(base + r * (64 * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
+      const int left = end - m - chunk * VEC;
+      if (r0 + r >= a.N || left <= 0) continue;
+      Y* const y = static_cast<Y*>(a.y) + (r0 + r) * a.ldy + m + chunk * VEC;
+      if (a.wide_out && left >= VEC) {
+        __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(y));   // nobody reads them here: the L2 keeps x and the weights
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (e < left) {
+            if constexpr (sizeof(Y) == 4) y[e] = __uint_as_float((uint32_t)v[e]);
+            else y[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
+          }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
 // ------------------------------------------------------------------------------------------------------------- rows
 // A wave owns 16 rows at a time.  Lane (row i = lane % 16, group g = lane / 16) holds 16 values of every step of 64
 // columns.  Which 16 is free as long as both operands agree, so they are the ones that make the loads whole: in float32
 // columns 16 p + 4 g .. + 3 (a row's four groups read 64 consecutive bytes per load), in bfloat16 32 p + 8 g .. + 7, in
 // 8 bits 16 g .. + 15; the weights are brought into that order on their way to LDS, once per block.
-// A result tile leaves lane (row, g) with the tile's weight rows 4 g .. 4 g + 3.  float32 results leave as they are, 16
-// bytes per lane and 64 consecutive ones per row and store; for bfloat16 the weight rows of a pair of tiles t are laid so
-// that a lane ends with 8 consecutive outputs: column 8 (i / 4) + 4 t + i % 4 of the pair in row 16 t + i.
+// A result tile leaves lane (row, g) with the tile's weight rows 4 g .. 4 g + 3; the weight rows of a pair of tiles t are
+// laid so that a lane ends with 8 consecutive outputs: column 8 (i / 4) + 4 t + i % 4 of the pair in row 16 t + i.
 constexpr int kI8RowsThreads = 512;
-constexpr int kI8RowsLds = 144 * 1024;
+constexpr int kI8RowsLds = 120 * 1024;   // for weights, their scales and biases; the result patches come on top
 
 template <typename X> struct XRaw;
 template <> struct XRaw<float> { float v[16]; };
@@ -164,6 +203,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
   const int Kp = (a.K + 15) & ~15, steps = (a.K + 63) >> 6;
   float* const s_ws = reinterpret_cast<float*>(lds + m_pad * PITCH);
   float* const s_bias = s_ws + m_pad;
+  const Patch<Y, 16> patch{reinterpret_cast<char*>(s_bias + m_pad) + wave * (int)Patch<Y, 16>::BYTES};
   const X* const x = static_cast<const X*>(a.x);
 
   const int64_t tiles = (a.N + 15) >> 4, step = (int64_t)gridDim.x * (kI8RowsThreads / 64);
@@ -185,7 +225,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
     const int pos = idx / (KS * 4), c = idx - pos * (KS * 4);
     if (16 * c >= Kp) continue;         // never multiplied by anything but zeros
     const int r = pos & 15;
-    const int m = m_begin + (sizeof(Y) == 4 ? pos : (pos & ~31) + 8 * (r >> 2) + 4 * ((pos >> 4) & 1) + (r & 3));
+    const int m = m_begin + (pos & ~31) + 8 * (r >> 2) + 4 * ((pos >> 4) & 1) + (r & 3);
     const i32x4 v = *reinterpret_cast<const i32x4*>(a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw + 16 * c);
     char* d = lds + pos * PITCH + (c >> 2) * 64;
     const int cc = c & 3;
@@ -255,9 +295,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
           }
         }
     }
-    const int64_t row = 16 * tile + i;
     if (tile + step < tiles) fetch(tile + step);
-    Y* const y = static_cast<Y*>(a.y) + row * a.ldy + m_begin;
     for (int b = 0; b < m_pad; b += 32) {
       i32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
       const char* w = lds + (b + i) * PITCH + g * 16;
@@ -267,26 +305,24 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
 #pragma unroll
           for (int t = 0; t < 2; ++t)
             acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(w + t * 16 * PITCH + s * 64), q[s], acc[t], 0, 0, 0);
-      float v[2][4];
-      auto first_of = [&](int t) { return b + (sizeof(Y) == 4 ? 16 * t + 4 * g : 8 * g + 4 * t); };
+      float v[8];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const float4 ws = *reinterpret_cast<const float4*>(s_ws + first_of(t));
-        const float4 bs = *reinterpret_cast<const float4*>(s_bias + first_of(t));
-        v[t][0] = finish(acc[t][0], xs * ws.x, bs.x, a.relu);
-        v[t][1] = finish(acc[t][1], xs * ws.y, bs.y, a.relu);
-        v[t][2] = finish(acc[t][2], xs * ws.z, bs.z, a.relu);
-        v[t][3] = finish(acc[t][3], xs * ws.w, bs.w, a.relu);
+        const float4 ws = *reinterpret_cast<const float4*>(s_ws + b + 8 * g + 4 * t);
+        const float4 bs = *reinterpret_cast<const float4*>(s_bias + b + 8 * g + 4 * t);
+        v[4 * t] = finish(acc[t][0], xs * ws.x, bs.x, a.relu);
+        v[4 * t + 1] = finish(acc[t][1], xs * ws.y, bs.y, a.relu);
+        v[4 * t + 2] = finish(acc[t][2], xs * ws.z, bs.z, a.relu);
+        v[4 * t + 3] = finish(acc[t][3], xs * ws.w, bs.w, a.relu);
       }
-      if (row < a.N) {
-        if constexpr (sizeof(Y) == 4) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) store_outputs<Y, 4>(y + first_of(t), v[t], m_count - first_of(t), a.wide_out);
-        } else {
-          const float w[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
-          store_outputs<Y, 8>(y + b + 8 * g, w, m_count - b - 8 * g, a.wide_out);
-        }
+      const int chunk = ((b & 32) + 8 * g) / patch.VEC;
+      if constexpr (sizeof(Y) == 4) {
+        patch.put(i, chunk, {v[0], v[1], v[2], v[3]});
+        patch.put(i, chunk + 1, {v[4], v[5], v[6], v[7]});
+      } else {
+        patch.put(i, chunk, v);
       }
+      if ((b & 32) || b + 32 >= m_pad) patch.leave(a, 16 * tile, m_begin + (b & ~63), m_begin + m_count);
     }
   }
 }
@@ -341,7 +377,7 @@ __global__ void __launch_bounds__(kBlock) k_linear_i8_thin(I8Args a) {
 __device__ const i32x4 kZeroPiece = {0, 0, 0, 0};
 
 template <int WN, int WM, int TN, int PC>
-constexpr int tiles_lds() { return 2 * (WN * TN * 32 + WM * 64) * 16 * PC; }
+constexpr int tiles_lds() { return 2 * (WN * TN * 32 + WM * 64) * 16 * PC + 2 * WM * 64 * 4; }   // + scales and biases
 
 // Piece c of row r lies at this place of the row.
 template <int PC>
@@ -351,9 +387,8 @@ template <typename Y, int WN, int WM, int TN, int PC>
 __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, int n_tiles, int m_tiles) {
   constexpr int BN = WN * TN * 32, BM = WM * 64, WAVES = WN * WM;
   constexpr int ROW = 16 * PC, STAGE = (BN + BM) * ROW;
-  // results leave through the buffer that was read last: per wave 32 rows x 64 outputs
-  constexpr int VEC = 16 / sizeof(Y), CHUNKS = 64 / VEC, PATCH = 32 * 64 * sizeof(Y);
-  static_assert(WAVES * PATCH <= STAGE, "result patches fit a buffer");
+  // results leave through the buffer that was read last
+  static_assert(WAVES * Patch<Y, 32>::BYTES <= STAGE, "result patches fit a buffer");
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i32 = lane & 31, half = lane >> 5;
@@ -365,22 +400,27 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
   const int Kp = (a.K + 15) & ~15, pieces = Kp >> 4;
 
   // copies: one instruction of a wave fills 64 / PC rows (1 KiB); rows 0 .. BN - 1 are x's, the others weights
-  constexpr int COPIES = (BN + BM) * PC / 64 / WAVES;
-  const int8_t* src[COPIES];
+  constexpr int COPIES = (BN + BM) * PC / 64 / WAVES, COPIES_X = BN * PC / 64 / WAVES;
+  static_assert(COPIES_X * WAVES * 64 == BN * PC, "a copy is x's or the weights'");
+  const int8_t *x0 = nullptr, *w0 = nullptr;   // the tile's first rows, and the lane's rows from there
+  uint32_t from[COPIES];
   auto take = [&](int t) __attribute__((always_inline)) {   // false: no such tile
     const int nt = (t / m_tiles) * 8 + xcd;
     if (nt >= n_tiles) return false;
     const int64_t n0 = (int64_t)nt * BN;
     const int m0 = t % m_tiles * BM;
+    x0 = static_cast<const int8_t*>(a.x) + n0 * a.ldx;
+    w0 = a.w + (int64_t)m0 * a.ldw;
+    const int n_last = a.N - n0 < BN ? (int)(a.N - n0) - 1 : BN - 1, m_last = a.M - m0 < BM ? a.M - m0 - 1 : BM - 1;
 #pragma unroll
     for (int c = 0; c < COPIES; ++c) {
       const int r = (c * WAVES + wave) * (64 / PC) + lane / PC;
-      if (r < BN) {
-        src[c] = static_cast<const int8_t*>(a.x) + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldx;
+      if (c < COPIES_X) {
+        from[c] = (uint32_t)(r < n_last ? r : n_last) * (uint32_t)a.ldx;
       } else {
         const int p = r - BN, i = p & 31;
-        const int m = m0 + (p & ~63) + 32 * ((i >> 2) & 1) + 16 * ((p >> 5) & 1) + 4 * (i >> 3) + (i & 3);
-        src[c] = a.w + (int64_t)(m < a.M ? m : a.M - 1) * a.ldw;
+        const int m = (p & ~63) + 32 * ((i >> 2) & 1) + 16 * ((p >> 5) & 1) + 4 * (i >> 3) + (i & 3);
+        from[c] = (uint32_t)(m < m_last ? m : m_last) * (uint32_t)a.ldw;
       }
     }
     return true;
@@ -390,8 +430,8 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
     const int at = p0 + piece;
 #pragma unroll
     for (int c = 0; c < COPIES; ++c) {
-      const int8_t* from = at < pieces ? src[c] + 16 * at : reinterpret_cast<const int8_t*>(&kZeroPiece);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+      const int8_t* p = at < pieces ? (c < COPIES_X ? x0 : w0) + (from[c] + 16 * at) : reinterpret_cast<const int8_t*>(&kZeroPiece);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
                                        (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (c * WAVES + wave) * 1024), 16, 0, 0);
     }
   };
@@ -403,6 +443,20 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
     const int64_t n0 = (int64_t)((tile / m_tiles) * 8 + xcd) * BN;
     const int m0 = tile % m_tiles * BM;
     tile += turn;
+    // What the results need besides the sums is loaded here, ahead of a barrier that waits for everything.  While copies
+    // to LDS are on their way nothing is loaded into registers and nothing may be spilled: values that were reloaded
+    // under them came out wrong now and then.
+    float xs[TN], ws = 0.f, bs = 0.f;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int64_t row = n0 + (wn * TN + j) * 32 + i32;
+      xs[j] = a.xs[row < a.N ? row : a.N - 1];
+    }
+    if (threadIdx.x < BM) {
+      const int m = m0 + (int)threadIdx.x < a.M ? m0 + (int)threadIdx.x : a.M - 1;
+      ws = a.ws[m];
+      if (a.bias) bs = scalar_to_f32(static_cast<const Y*>(a.bias)[m]);
+    }
     i32x16 acc[TN][2];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -416,84 +470,60 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
       else if ((more = take(tile))) stage(buf ^ 1, 0);
       const char* const xb = lds + buf * STAGE + (wn * TN * 32 + i32) * ROW;
       const char* const wb = lds + buf * STAGE + (BN + wm * 64 + i32) * ROW;
-      const bool partial = (a.K & 15) && p0 + PC >= pieces;
-#pragma unroll
-      for (int kk = 0; kk < PC / 2; ++kk) {
+      if ((a.K & 15) && p0 + PC >= pieces) {   // the last piece holds bytes that are no columns
+        for (int r = threadIdx.x; r < BN; r += WAVES * 64) {
+          i32x4* const p = reinterpret_cast<i32x4*>(lds + buf * STAGE + r * ROW + piece_at<PC>(r, pieces - 1 - p0) * 16);
+          *p = keep_bytes(*p, a.K & 15);
+        }
+        __syncthreads();
+      }
+      i32x4 w[2][2], v[2][TN];                 // the operands of one product are on their way while the one before runs
+      auto read = [&](auto kk) __attribute__((always_inline)) {
         const int slot = piece_at<PC>(lane, 2 * kk + half) * 16;
-        i32x4 w[2], v[TN];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) w[t] = *reinterpret_cast<const i32x4*>(wb + t * 32 * ROW + slot);
+        for (int t = 0; t < 2; ++t) w[kk % 2][t] = *reinterpret_cast<const i32x4*>(wb + t * 32 * ROW + slot);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) v[j] = *reinterpret_cast<const i32x4*>(xb + j * 32 * ROW + slot);
-        if (partial)
-#pragma unroll
-          for (int j = 0; j < TN; ++j) v[j] = keep_bytes(v[j], a.K - 16 * (p0 + 2 * kk + half));
+        for (int j = 0; j < TN; ++j) v[kk % 2][j] = *reinterpret_cast<const i32x4*>(xb + j * 32 * ROW + slot);
+      };
+      read(std::integral_constant<int, 0>{});
+      each<PC / 2>([&](auto kk) __attribute__((always_inline)) {
+        if constexpr (kk + 1 < PC / 2) read(std::integral_constant<int, kk + 1>{});
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[t], v[j], acc[j][t], 0, 0, 0);
-      }
+          for (int t = 0; t < 2; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[kk % 2][t], v[kk % 2][j], acc[j][t], 0, 0, 0);
+      });
     }
-    // scales and biases of the lane's 32 outputs, the same for every row
-    const int mw = m0 + wm * 64, mb = mw + 32 * half;
-    float ws[32], bs[32];
-    if (mw + 64 <= a.M && a.wide_vectors) {
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const float4 t = *reinterpret_cast<const float4*>(a.ws + mb + e);
-        ws[e] = t.x; ws[e + 1] = t.y; ws[e + 2] = t.z; ws[e + 3] = t.w;
-        float u[4] = {0.f, 0.f, 0.f, 0.f};
-        if (a.bias) EdgeIO<Y, 4>::load(static_cast<const Y*>(a.bias) + mb + e, u);
-        bs[e] = u[0]; bs[e + 1] = u[1]; bs[e + 2] = u[2]; bs[e + 3] = u[3];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int m = mb + e < a.M ? mb + e : a.M - 1;
-        ws[e] = a.ws[m];
-        bs[e] = a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[m]) : 0.f;
-      }
+    float* const s_ws = reinterpret_cast<float*>(lds + 2 * STAGE);
+    float* const s_bs = s_ws + BM;
+    if (threadIdx.x < BM) {
+      s_ws[threadIdx.x] = ws;
+      s_bs[threadIdx.x] = bs;
     }
+    const int mw = m0 + wm * 64;
     __syncthreads();                       // every wave has read its operands: the buffer may take results
-    char* const patch = lds + (buf ^ 1) * STAGE + wave * PATCH;
+    const Patch<Y, 32> patch{lds + (buf ^ 1) * STAGE + wave * (int)Patch<Y, 32>::BYTES};
+    constexpr int VEC = Patch<Y, 32>::VEC;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int64_t r0 = n0 + (wn * TN + j) * 32;
-      const float xs = a.xs[r0 + i32 < a.N ? r0 + i32 : a.N - 1];
-      // 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread
 #pragma unroll
       for (int c = 0; c < 32 / VEC; ++c) {
-        float v[VEC];
+        float v[VEC], sw[VEC], sb[VEC];
+        const int first = wm * 64 + 32 * half + c * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+          const float4 t = *reinterpret_cast<const float4*>(s_ws + first + e), u = *reinterpret_cast<const float4*>(s_bs + first + e);
+          sw[e] = t.x; sw[e + 1] = t.y; sw[e + 2] = t.z; sw[e + 3] = t.w;
+          sb[e] = u.x; sb[e + 1] = u.y; sb[e + 2] = u.z; sb[e + 3] = u.w;
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const int o = c * VEC + e;
-          v[e] = finish(acc[j][o >> 4][o & 15], xs * ws[o], bs[o], a.relu);
+          v[e] = finish(acc[j][o >> 4][o & 15], xs[j] * sw[e], sb[e], a.relu);
         }
-        const int chunk = half * (32 / VEC) + c;
-        store_outputs<Y, VEC>(reinterpret_cast<Y*>(patch + i32 * (64 * (int)sizeof(Y)) + ((chunk ^ i32) & (CHUNKS - 1)) * 16), v, VEC, true);
+        patch.put(i32, half * (32 / VEC) + c, v);
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int q = 0; q < 32 * CHUNKS / 64; ++q) {
-        const int r = q * (64 / CHUNKS) + lane / CHUNKS, chunk = lane % CHUNKS;
-        const i32x4 v = *reinterpret_cast<const i32x4*>(patch + r * (64 * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
-        const int left = a.M - mw - chunk * VEC;
-        if (r0 + r >= a.N || left <= 0) continue;
-        Y* const y = static_cast<Y*>(a.y) + (r0 + r) * a.ldy + mw + chunk * VEC;
-        if (a.wide_out && left >= VEC) {
-          *reinterpret_cast<i32x4*>(y) = v;
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (e < left) {
-              if constexpr (sizeof(Y) == 4) y[e] = __uint_as_float((uint32_t)v[e]);
-              else y[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
-            }
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      patch.leave(a, n0 + (wn * TN + j) * 32, mw, a.M);
     }
   }
 }
@@ -520,7 +550,7 @@ int32_t launch_rows(const I8Args& a, hipStream_t stream) {
   while (slices < m32 && row_blocks * slices < 256) ++slices;
   int per = (m32 + slices - 1) / slices;
   slices = (m32 + per - 1) / per;
-  const int bytes = per * per32;
+  const int bytes = per * per32 + kI8RowsThreads / 64 * (int)Patch<Y, 16>::BYTES;
   int per_cu = 160 * 1024 / bytes;
   const int by_regs = rows_waves<X>(KS) / 2;
   if (per_cu > by_regs) per_cu = by_regs;
@@ -547,13 +577,19 @@ template <typename Y, int WN, int WM, int TN, int PC>
 int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
   constexpr int BN = WN * TN * 32, BM = WM * 64, bytes = tiles_lds<WN, WM, TN, PC>();
   const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
+  if (a.ldx > kI8MaxTileLd || a.ldw > kI8MaxTileLd) return fail(MPNN_E_INVALID, "mpnn_linear_int8: row strides above %d", kI8MaxTileLd);
   const int64_t all = (nt + 7) / 8 * 8 * mt;
   const int64_t resident = 256 * (160 * 1024 / bytes);
   const int64_t grid = all < resident ? all : resident;
   if (all > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld M=%d", (long long)a.N, a.M);
-  if (bytes > 64 * 1024)
-    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_tiles<Y, WN, WM, TN, PC>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  const void* const f = reinterpret_cast<const void*>(k_linear_i8_tiles<Y, WN, WM, TN, PC>);
+  static const hipError_t sound = [f] {   // a build that had to spill registers is not run (see the kernel)
+    hipFuncAttributes attr;
+    const hipError_t e = hipFuncGetAttributes(&attr, f);
+    return e != hipSuccess ? e : (attr.localSizeBytes != 0 ? hipErrorInvalidKernelFile : hipSuccess);
+  }();
+  MPNN_HIP_CHECK(sound);
+  MPNN_HIP_CHECK(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
   k_linear_i8_tiles<Y, WN, WM, TN, PC><<<(unsigned)grid, WN * WM * 64, bytes, stream>>>(a, (int)nt, (int)mt);
   MPNN_LAUNCH_CHECK("k_linear_i8_tiles");
   return MPNN_OK;
@@ -574,7 +610,7 @@ int32_t launch_i8(const I8Args& a, I8Kernel kernel, int x_dtype, bool wide_in, h
     return MPNN_OK;
   }
   // tiles of 256 x 256 if they fill the CUs, of 128 x 128 otherwise
-  if (((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, I8BIG>(a, stream);
+  if (((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, 2, 4, 4, 8>(a, stream);
   return launch_tiles<Y, 2, 2, 2, 8>(a, stream);
 }
 
@@ -610,8 +646,7 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
   if ((N + 31) / 32 > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld", (long long)N);
   const int vec = y_dtype == MPNN_BF16 ? 8 : 4;
   const int wide_out = ((uintptr_t)Y & 15) == 0 && ldy % vec == 0;
-  const int wide_vectors = (((uintptr_t)w_scale | (uintptr_t)bias) & 15) == 0;
-  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out, wide_vectors};
+  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out};
   if (take) {
     int8_t* q = static_cast<int8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + N * Kp);

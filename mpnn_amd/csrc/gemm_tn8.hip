@@ -16,8 +16,6 @@
 //          value is converted once per block.  Column 4 i + t of a tile is column i of matrix tile t.
 //   strips x tiles < 8: the waves left over share the rows of a slab; their sums meet in LDS at the end, in wave order.
 // One partial tile per block, added in block order by a second launch: no atomics, the same bits on every run.
-#include <utility>
-
 #include "common.h"
 #include "rowio.h"
 
@@ -86,16 +84,6 @@ __device__ __forceinline__ void pieces_of(const float (&v)[8], bf16x8 (&out)[P])
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
   }
-}
-
-// f(0), f(1), .. f(N - 1) with the index known where the registers it picks are named.
-template <typename F, int... I>
-__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each(F&& f) {
-  each_of(f, std::make_integer_sequence<int, N>{});
 }
 
 // T: float (strips of 32 columns, one matrix tile per wave and column tile) or bf16_t (64 columns: a lane loads columns

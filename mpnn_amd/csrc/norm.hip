@@ -102,13 +102,6 @@ struct RowSum {
   }
 };
 
-// Two floats to packed bfloat16, nearest even (one instruction).
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, bf16x2_t));
-}
-
 // VEC columns of T at a time: 16 bytes in float32, 8 in bfloat16, or one column.
 template <typename T, int VEC>
 struct NormIO : RowIO<T, VEC> {};

@@ -49,13 +49,16 @@ class Rows8:
         return (self.values.float() * self.scale.unsqueeze(1)).to(dtype)
 
 
+_MAX_PITCH = 1 << 21     # bytes (8-bit rows) or elements (their partners in gemm_tn8) from row to row
+
+
 def _pitch(k: int) -> int:
     return (k + 15) // 16 * 16
 
 
 def _in_place(v: torch.Tensor) -> bool:
     n, k = v.shape
-    if v.data_ptr() % 16 or (k > 1 and v.stride(1) != 1) or (n > 1 and (v.stride(0) % 16 or v.stride(0) < _pitch(k))):
+    if v.data_ptr() % 16 or (k > 1 and v.stride(1) != 1) or (n > 1 and (v.stride(0) % 16 or not _pitch(k) <= v.stride(0) <= _MAX_PITCH)):
         return False
     # the last row's 16-byte pieces must lie inside the storage
     end = v.storage_offset() + (max(n, 1) - 1) * v.stride(0) + _pitch(k)
@@ -147,9 +150,6 @@ def relu_bits(y: torch.Tensor) -> torch.Tensor:
     _lib.check(_lib.load().mpnn_relu_bits(_lib.ptr(y), _lib.leading(y), _lib.dtype_code(y.dtype), n, m, _lib.ptr(bits),
                                           _lib.stream_handle(y.device)), "mpnn_relu_bits")
     return bits
-
-
-_MAX_PITCH = 1 << 21     # of gemm_tn8's operands
 
 
 def gemm_tn8(g: torch.Tensor, x: Rows8, x2: Rows8 | None = None, bits=None, g_out=None) -> torch.Tensor:
