@@ -16,6 +16,10 @@
 //          value is converted once per block.  Column 4 i + t of a tile is column i of matrix tile t.
 //   strips x tiles < 8: the waves left over share the rows of a slab; their sums meet in LDS at the end, in wave order.
 // One partial tile per block, added in block order by a second launch: no atomics, the same bits on every run.
+// Measured on 4 M rows: float32 256 x 128 0.97 ms = 4.8 TB/s, 128 x [128 | 128] with the relu's bits and g * open
+// written 1.13 ms = 4.6 TB/s; bfloat16 256 x 128 0.63 ms = 4.1 TB/s, 128 x [128 | 128] with both 0.90 ms = 3.5 TB/s (a
+// copy reaches 4.9).  What bounds bfloat16 there: the pieces are made once per matrix of q for half the bytes of g.
+// Slabs of 64 rows instead of 128 for two column tiles took 1.13 ms, row clamps instead of whole slabs 20 % more.
 #include "common.h"
 #include "rowio.h"
 
@@ -28,7 +32,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTn8Threads = 512;
 constexpr int kTn8MaxLd = 1 << 21;     // row strides: 24-bit byte offsets times a row of the slab fit 32 bits
-constexpr int kTn8LdsBytes = 65536;   // two buffers of 128 rows x 128 columns (or 64 rows x two tiles) in bfloat16
+constexpr int kTn8Rows = 128;           // rows per slab
+constexpr int kTn8Tile = kTn8Rows * 256;   // bytes of a column tile of a slab: 128 columns in bfloat16
+constexpr int tn8_lds(int wk) { return 2 * wk * kTn8Tile + 2 * wk * kTn8Rows * 4; }
 
 struct Tn8Args {
   const void* g;
@@ -61,7 +67,8 @@ __device__ __forceinline__ u32x4 column_of(const uint32_t (&w)[8], int t) {
   return r;
 }
 
-// The pieces of 8 products: each piece is the upper half of what is left, so that the difference is exact.
+// The pieces of 8 products.  Three: each is the upper half of what is left, so that the differences are exact and the
+// third takes the rest whole.  Two: the nearest bfloat16 and the nearest to the exact difference, 2^-17 of the product.
 template <int P>
 __device__ __forceinline__ void pieces_of(const float (&v)[8], bf16x8 (&out)[P]) {
   float r[8];
@@ -71,18 +78,16 @@ __device__ __forceinline__ void pieces_of(const float (&v)[8], bf16x8 (&out)[P])
   for (int p = 0; p < P; ++p) {
     u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t lo = __float_as_uint(r[2 * j]), hi = __float_as_uint(r[2 * j + 1]);
-      if (P == 2 && p == 1) {   // the last of two pieces is rounded (half up); the third of three is exact
-        lo += 0x8000u;
-        hi += 0x8000u;
-      }
-      w[j] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-    }
+    for (int j = 0; j < 4; ++j)
+      w[j] = P == 2 ? pack_bf16(r[2 * j], r[2 * j + 1])
+                    : __builtin_amdgcn_perm(__float_as_uint(r[2 * j + 1]), __float_as_uint(r[2 * j]), 0x07060302u);
     out[p] = __builtin_bit_cast(bf16x8, w);
     if (p + 1 < P)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
+      for (int j = 0; j < 4; ++j) {
+        r[2 * j] -= __uint_as_float(P == 2 ? w[j] << 16 : __float_as_uint(r[2 * j]) & 0xffff0000u);
+        r[2 * j + 1] -= __uint_as_float(P == 2 ? w[j] & 0xffff0000u : __float_as_uint(r[2 * j + 1]) & 0xffff0000u);
+      }
   }
 }
 
@@ -93,12 +98,12 @@ __global__ void __launch_bounds__(kTn8Threads, 2) k_gemm_tn8(Tn8Args a) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int U = BF ? 2 : 1;              // matrix tiles of g's columns per wave
   constexpr int P = BF ? 2 : 3;              // pieces
-  constexpr int SN = 128 / WK;               // rows per slab
+  constexpr int SN = kTn8Rows;
   constexpr int STEPS = SN / 16 / WN;        // of this wave per slab
-  constexpr int D = STEPS < (BF ? 2 : 4) ? STEPS : (BF ? 2 : 4);   // steps of g in flight, 2 KiB per wave each
+  constexpr int D = STEPS < 4 ? STEPS : 4;   // steps of g in flight, 2 KiB per wave each
   static_assert(WM * WK * WN == 8 && STEPS >= 1, "8 waves");
-  __shared__ __attribute__((aligned(16))) char smem[kTn8LdsBytes];
-  __shared__ float s_scale[2][2][128];
+  extern __shared__ __align__(16) char smem[];
+  float* const s_scale = reinterpret_cast<float*>(smem + 2 * WK * kTn8Tile);   // [2][WK][SN]
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform: what hangs on it stays in scalar registers
   const int i32 = lane & 31, half = lane >> 5;
@@ -117,48 +122,60 @@ __global__ void __launch_bounds__(kTn8Threads, 2) k_gemm_tn8(Tn8Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[u][t][r] = 0.f;
 
-  // staging: thread -> (tile of the block, octet of rows, word of 4 columns); 16 octets x 32 words (one tile) or
-  // 2 tiles x 8 octets x 32 words = 512 threads
-  const int st_tile = WK == 2 ? tid >> 8 : 0;
-  const int st_oct = WK == 2 ? (tid >> 5) & 7 : tid >> 5;
-  const int st_word = tid & 31;
-  const int st_t = (int)blockIdx.z * WK + st_tile < a.ktiles ? (int)blockIdx.z * WK + st_tile : 0;
-  const bool st_second = st_t >= z0;
-  const int8_t* st_q = st_second ? a.q2 : a.q;
-  const int64_t st_ld = st_second ? a.ldq2 : a.ldq;
-  const float* st_scale = st_second ? a.scale2 : a.scale;
-  int st_col = (st_second ? st_t - z0 : st_t) * 128 + 4 * st_word;
-  if (st_col >= ((st_second ? a.K2 : a.K) + 15) / 16 * 16) st_col = 0;   // past the row: any bytes, never stored
-  uint32_t qw[8];
+  // In float32 the sums of 1024 rows at a time are added to a second set: one chain over all of a block's rows would lose
+  // two digits on millions of rows (a product's rounding to bfloat16 hides that).
+  constexpr int CHAIN = 8;                   // slabs
+  f32x16 whole[BF ? 1 : U][BF ? 1 : 4];
+  int chain = 0;
+  if constexpr (!BF)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) whole[0][t] = acc[0][t];
+
+  // staging: thread -> (octet of rows, word of 4 columns), 16 x 32 for each of the block's tiles
+  const int st_oct = tid >> 5, st_word = tid & 31;
+  const int8_t* st_q[WK];
+  const float* st_scale[WK];
+  int64_t st_ld[WK];
+  uint32_t st_col[WK], q_off[WK];
+#pragma unroll
+  for (int w = 0; w < WK; ++w) {
+    const int t = (int)blockIdx.z * WK + w < a.ktiles ? (int)blockIdx.z * WK + w : 0;
+    const bool second = t >= z0;
+    st_q[w] = second ? a.q2 : a.q;
+    st_ld[w] = second ? a.ldq2 : a.ldq;
+    st_scale[w] = second ? a.scale2 : a.scale;
+    const int col = (second ? t - z0 : t) * 128 + 4 * st_word;
+    st_col[w] = col < ((second ? a.K2 : a.K) + 15) / 16 * 16 ? col : 0;   // past the row: any bytes, never stored
+    q_off[w] = __umul24(8 * st_oct, (uint32_t)st_ld[w]) + st_col[w];
+  }
+  uint32_t qw[WK][8];
   float sc = 0.f;
-  // Addresses: a uniform base per row and 32-bit offsets from it (row strides are bounded by the host).  Rows past the
-  // end (of the last slab) are read at the last row and count with scale 0: finite values add nothing, and where that
-  // row holds an infinity or a NaN its own term has made the sum a NaN already.
-  auto last_of = [&](int64_t n0) { return (uint32_t)(a.N - n0 < SN ? a.N - n0 - 1 : SN - 1); };
-  const uint32_t q_off = __umul24(8 * st_oct, (uint32_t)st_ld) + st_col;
-  auto fetch_q = [&](int64_t n0) __attribute__((always_inline)) {
-    const uint32_t last = last_of(n0);
-    const int8_t* base = st_q + n0 * st_ld;
-    if (last == SN - 1) {
-      each<8>([&](auto j) __attribute__((always_inline)) { qw[j] = *reinterpret_cast<const uint32_t*>(base + j * st_ld + q_off); });
-    } else {
-      each<8>([&](auto j) __attribute__((always_inline)) {
-        uint32_t row = 8 * st_oct + j;
-        row = row < last ? row : last;
-        qw[j] = *reinterpret_cast<const uint32_t*>(base + (__umul24(row, (uint32_t)st_ld) + st_col));
-      });
+  // Every slab is whole: the last one starts SN rows before the end, and its rows that belong to the slab before count
+  // with scale 0 (finite values add nothing then; an infinity or a NaN has made its sums NaN in its own slab already).
+  // Addresses: a uniform base per row and 32-bit offsets from it (row strides are bounded by the host).
+  auto first_of = [&](int slab) { return (int64_t)slab * SN < a.N - SN ? (int64_t)slab * SN : a.N - SN; };
+  auto fetch_q = [&](int slab) __attribute__((always_inline)) {
+    const int64_t n0 = first_of(slab);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const int8_t* base = st_q[w] + n0 * st_ld[w];
+      each<8>([&](auto j) __attribute__((always_inline)) { qw[w][j] = *reinterpret_cast<const uint32_t*>(base + j * st_ld[w] + q_off[w]); });
     }
-    // the scales of the slab's rows: tile 0's by threads 0.., tile 1's by threads 256..
-    const uint32_t r = WK == 2 ? tid & 255 : tid;
-    if (r < SN) sc = r <= last ? st_scale[n0 + r] : 0.f;
+    // the scales of the slab's rows: tile 0's by the first 128 threads, tile 1's by the next
+    if (tid < WK * SN) {
+      const int64_t row = n0 + (tid & (SN - 1));
+      sc = row >= (int64_t)slab * SN ? (WK == 2 && tid >= SN ? st_scale[WK - 1] : st_scale[0])[row] : 0.f;
+    }
   };
   auto stash_q = [&](int buf) __attribute__((always_inline)) {
-    char* base = smem + buf * (kTn8LdsBytes / 2) + st_tile * (SN * 256);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      *reinterpret_cast<u32x4*>(base + ((((st_oct >> 1) * 4 + t) * 64) + (st_oct & 1) * 32 + st_word) * 16) = column_of(qw, t);
-    const int r = WK == 2 ? tid & 255 : tid;
-    if (r < SN) s_scale[buf][st_tile][r] = sc;
+    for (int w = 0; w < WK; ++w) {
+      char* base = smem + (buf * WK + w) * kTn8Tile;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        *reinterpret_cast<u32x4*>(base + ((((st_oct >> 1) * 4 + t) * 64) + (st_oct & 1) * 32 + st_word) * 16) = column_of(qw[w], t);
+    }
+    if (tid < WK * SN) s_scale[buf * WK * SN + tid] = sc;
   };
 
   // g: the lane's columns, 8 rows per step
@@ -172,28 +189,12 @@ __global__ void __launch_bounds__(kTn8Threads, 2) k_gemm_tn8(Tn8Args a) {
   const int64_t ldg = a.ldg * (int64_t)sizeof(T);
   const uint32_t g_off = __umul24(8 * half, (uint32_t)ldg) + gcol * sizeof(T);
   const uint32_t b_off = __umul24(8 * half + (lane & 7), (uint32_t)a.bits_pitch) + wbit_in;
-  auto fetch_g = [&](int64_t n0, auto s) __attribute__((always_inline)) {
-    const uint32_t last = last_of(n0);
-    const int step = wn + s * WN;
-    if (last == SN - 1) {
-      const char* base = static_cast<const char*>(a.g) + (n0 + step * 16) * ldg;
-      each<8>([&](auto j) __attribute__((always_inline)) { gr[s % D][j] = *reinterpret_cast<const uint32_t*>(base + j * ldg + g_off); });
-      // lane l of 8 holds the word of row l; the lanes trade them when they are used
-      if constexpr (BITS) br[s % D] = (a.bits + (n0 + step * 16) * a.bits_pitch)[b_off];
-    } else {
-      const uint32_t r0 = step * 16 + 8 * half;
-      const char* base = static_cast<const char*>(a.g) + n0 * ldg;
-      each<8>([&](auto j) __attribute__((always_inline)) {
-        uint32_t row = r0 + j;
-        row = row < last ? row : last;
-        gr[s % D][j] = *reinterpret_cast<const uint32_t*>(base + (__umul24(row, (uint32_t)ldg) + gcol * sizeof(T)));
-      });
-      if constexpr (BITS) {
-        uint32_t row = r0 + (lane & 7);
-        row = row < last ? row : last;
-        br[s % D] = (a.bits + n0 * a.bits_pitch)[__umul24(row, (uint32_t)a.bits_pitch) + wbit_in];
-      }
-    }
+  auto fetch_g = [&](int slab, auto s) __attribute__((always_inline)) {
+    const int64_t r0 = first_of(slab) + (wn + s * WN) * 16;
+    const char* base = static_cast<const char*>(a.g) + r0 * ldg;
+    each<8>([&](auto j) __attribute__((always_inline)) { gr[s % D][j] = *reinterpret_cast<const uint32_t*>(base + j * ldg + g_off); });
+    // lane l of 8 holds the word of row l; the lanes trade them when they are used
+    if constexpr (BITS) br[s % D] = (a.bits + r0 * a.bits_pitch)[b_off];
   };
 
   const int64_t ldgo = a.ldgo * (int64_t)sizeof(T);
@@ -201,44 +202,41 @@ __global__ void __launch_bounds__(kTn8Threads, 2) k_gemm_tn8(Tn8Args a) {
   int slab = blockIdx.x;
   int buf = 0;
   if (slab < a.slabs) {
-    const int64_t n0 = (int64_t)slab * SN;
-    fetch_q(n0);
-    if (live) each<D>([&](auto s) __attribute__((always_inline)) { fetch_g(n0, s); });
+    fetch_q(slab);
+    if (live) each<D>([&](auto s) __attribute__((always_inline)) { fetch_g(slab, s); });
     stash_q(0);
   }
   __syncthreads();
   for (; slab < a.slabs; slab += gridDim.x, buf ^= 1) {
-    const int64_t n0 = (int64_t)slab * SN;
     const int next = slab + (int)gridDim.x;
     const bool more = next < a.slabs;
-    if (more) fetch_q((int64_t)next * SN);
+    if (more) fetch_q(next);
     if (live) {
-      const char* base = smem + buf * (kTn8LdsBytes / 2) + wk * (SN * 256);
-      const uint32_t last = last_of(n0);
+      const char* base = smem + (buf * WK + wk) * kTn8Tile;
+      const float* const scales = s_scale + (buf * WK + wk) * SN;
       each<STEPS>([&](auto s) __attribute__((always_inline)) {
         const int step = wn + s * WN;
         uint32_t w[8];
         each<8>([&](auto j) __attribute__((always_inline)) {
           w[j] = gr[s % D][j];
           if constexpr (BITS) {
-            const uint32_t open = (uint32_t)__builtin_amdgcn_ds_swizzle((int)br[s % D], (j << 5) | 0x18) >> bshift;
-            if constexpr (BF) w[j] &= ((open & 1u) ? 0x0000ffffu : 0u) | ((open & 2u) ? 0xffff0000u : 0u);
-            else w[j] = (open & 1u) ? w[j] : 0u;
+            // one bit sign-extended is the mask of its entry
+            const int word = __builtin_amdgcn_ds_swizzle((int)br[s % D], (j << 5) | 0x18);
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe(word, bshift, 1);
+            if constexpr (BF) w[j] &= (lo & 0x0000ffffu) | ((uint32_t)__builtin_amdgcn_sbfe(word, bshift + 1, 1) & 0xffff0000u);
+            else w[j] &= lo;
           }
         });
         if (emit && col < a.M) {
-          char* out = static_cast<char*>(a.gout) + (n0 + step * 16) * ldgo;
-          const uint32_t r0 = step * 16 + 8 * half;
-          each<8>([&](auto j) __attribute__((always_inline)) {
-            if (r0 + j <= last) *reinterpret_cast<uint32_t*>(out + j * ldgo + o_off) = w[j];
-          });
+          char* out = static_cast<char*>(a.gout) + (first_of(slab) + step * 16) * ldgo;
+          each<8>([&](auto j) __attribute__((always_inline)) { *reinterpret_cast<uint32_t*>(out + j * ldgo + o_off) = w[j]; });
         }
-        if constexpr (s + D < STEPS) fetch_g(n0, std::integral_constant<int, s + D>{});
-        else if (more) fetch_g((int64_t)next * SN, std::integral_constant<int, s + D - STEPS>{});
+        if constexpr (s + D < STEPS) fetch_g(slab, std::integral_constant<int, s + D>{});
+        else if (more) fetch_g(next, std::integral_constant<int, s + D - STEPS>{});
         float sv[8];
         {
-          const float4 lo = *reinterpret_cast<const float4*>(&s_scale[buf][wk][step * 16 + 8 * half]);
-          const float4 hi = *reinterpret_cast<const float4*>(&s_scale[buf][wk][step * 16 + 8 * half + 4]);
+          const float4 lo = *reinterpret_cast<const float4*>(scales + step * 16 + 8 * half);
+          const float4 hi = *reinterpret_cast<const float4*>(scales + step * 16 + 8 * half + 4);
           sv[0] = lo.x; sv[1] = lo.y; sv[2] = lo.z; sv[3] = lo.w;
           sv[4] = hi.x; sv[5] = hi.y; sv[6] = hi.z; sv[7] = hi.w;
         }
@@ -264,9 +262,24 @@ __global__ void __launch_bounds__(kTn8Threads, 2) k_gemm_tn8(Tn8Args a) {
         __builtin_amdgcn_sched_barrier(0);   // steps are not mixed: their operands would not fit the registers
       });
     }
+    if constexpr (!BF) {
+      if (++chain == CHAIN || !more) {
+        chain = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            whole[0][t][r] += acc[0][t][r];
+            acc[0][t][r] = 0.f;
+          }
+      }
+    }
     if (more) stash_q(buf ^ 1);
     __syncthreads();
   }
+  if constexpr (!BF)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[0][t] = whole[0][t];
   // the row shares meet in LDS: share 1, 2, .. are added to share 0 in that order, 16 values per lane at a time
   if constexpr (WN > 1) {
     float* meet = reinterpret_cast<float*>(smem);      // [wave][16][64] floats: 4 KiB per wave
@@ -291,17 +304,17 @@ __global__ void __launch_bounds__(kTn8Threads, 2) k_gemm_tn8(Tn8Args a) {
   const bool second = my_t >= z0;
   const int k0 = (second ? my_t - z0 : my_t) * 128, km = second ? a.K2 : a.K, ktot = a.K + a.K2;
   float* out = a.partial + (int64_t)blockIdx.x * a.M * ktot + (second ? a.K : 0);
+  const int m_lane = m0 + 4 * half * U, k_lane = k0 + 4 * i32;
+  const uint32_t o_lane = (uint32_t)m_lane * (uint32_t)ktot + k_lane;   // M * ktot is bounded by the host
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int k = k0 + 4 * i32 + t;
+    for (int r = 0; r < 16; ++r) {
+      const int i = ((r & 3) + 8 * (r >> 2)) * U + u;   // + 4 U half: the tile's row
+      if (m_lane + i < a.M)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = (r & 3) + 8 * (r >> 2) + 4 * half;
-        const int m = m0 + i * U + u;
-        if (m < a.M && k < km) out[(int64_t)m * ktot + k] = acc[u][t][r];
-      }
+        for (int t = 0; t < 4; ++t)
+          if (k_lane + t < km) (out + (int64_t)i * ktot)[o_lane + t] = acc[u][t][r];
     }
 }
 
@@ -325,6 +338,29 @@ __global__ void __launch_bounds__(kBlock) k_tn8_sums(const float* __restrict__ p
     dW[(i / K) * ldw + (i % K)] = f32_to_scalar<T>((red[o] + red[64 + o]) + (red[128 + o] + red[192 + o]));
 }
 
+// Fewer rows than a slab: a thread per output, 64 consecutive columns of [q | q2] by 4 rows of dW to a block; float32
+// throughout.  Bound by latency.
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_gemm_tn8_few(Tn8Args a, T* __restrict__ dW, int64_t ldw) {
+  const int ktot = a.K + a.K2;
+  const int c = (int)blockIdx.x * 64 + (threadIdx.x & 63), m = (int)blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (m >= a.M) return;
+  const bool second = c >= a.K;
+  const int8_t* q = second ? a.q2 : a.q;
+  const int64_t ldq = second ? a.ldq2 : a.ldq;
+  const float* scale = second ? a.scale2 : a.scale;
+  const int k = c < ktot ? (second ? c - a.K : c) : 0;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int n = 0; n < (int)a.N; ++n) {
+    float g = scalar_to_f32(static_cast<const T*>(a.g)[(int64_t)n * a.ldg + m]);
+    if (a.bits && !((a.bits[(int64_t)n * a.bits_pitch + (m >> 5)] >> (m & 31)) & 1u)) g = 0.f;
+    if (a.gout && c == 0) static_cast<T*>(a.gout)[n * a.ldgo + m] = f32_to_scalar<T>(g);
+    if (c < ktot) sum = fmaf(g * scale[n], (float)q[n * ldq + k], sum);
+  }
+  if (c < ktot) dW[m * ldw + c] = f32_to_scalar<T>(sum);
+}
+
 struct Tn8Plan {
   int wm, wk, wn, strips, ktiles, slab_rows, blocks;
 };
@@ -338,7 +374,7 @@ Tn8Plan tn8_plan(int64_t N, int M, int K, int K2, bool bf16) {
   p.wm = p.strips > 4 ? 8 : (p.strips > 2 ? 4 : p.strips);
   p.wk = (p.ktiles > 1 && p.wm < 8) ? 2 : 1;
   p.wn = 8 / (p.wm * p.wk);
-  p.slab_rows = 128 / p.wk;
+  p.slab_rows = kTn8Rows;
   // one block per CU over all output tiles, at least two slabs each
   const int tiles = ((p.strips + p.wm - 1) / p.wm) * ((p.ktiles + p.wk - 1) / p.wk);
   int64_t blocks = 256 / tiles;
@@ -349,15 +385,21 @@ Tn8Plan tn8_plan(int64_t N, int M, int K, int K2, bool bf16) {
   return p;
 }
 
+int32_t launch_one(void (*kernel)(Tn8Args), const Tn8Args& a, dim3 grid, int wk, hipStream_t stream) {
+  const int bytes = tn8_lds(wk);
+  MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  kernel<<<grid, kTn8Threads, bytes, stream>>>(a);
+  MPNN_LAUNCH_CHECK("k_gemm_tn8");
+  return MPNN_OK;
+}
+
 template <typename T>
-bool launch_tn8(const Tn8Args& a, const Tn8Plan& p, hipStream_t stream) {
+int32_t launch_tn8(const Tn8Args& a, const Tn8Plan& p, hipStream_t stream) {
   const dim3 grid(p.blocks, (p.strips + p.wm - 1) / p.wm, (p.ktiles + p.wk - 1) / p.wk);
-#define MPNN_TN8(WM, WK, WN) \
-  if (p.wm == WM && p.wk == WK) {                                                          \
-    if (a.bits) k_gemm_tn8<T, WM, WK, WN, true><<<grid, kTn8Threads, 0, stream>>>(a);      \
-    else k_gemm_tn8<T, WM, WK, WN, false><<<grid, kTn8Threads, 0, stream>>>(a);            \
-    return true;                                                                           \
-  }
+#define MPNN_TN8(WM, WK, WN)                                                              \
+  if (p.wm == WM && p.wk == WK)                                                           \
+    return a.bits ? launch_one(k_gemm_tn8<T, WM, WK, WN, true>, a, grid, WK, stream)      \
+                  : launch_one(k_gemm_tn8<T, WM, WK, WN, false>, a, grid, WK, stream);
   MPNN_TN8(8, 1, 1)
   MPNN_TN8(4, 1, 2)
   MPNN_TN8(4, 2, 1)
@@ -366,7 +408,7 @@ bool launch_tn8(const Tn8Args& a, const Tn8Plan& p, hipStream_t stream) {
   MPNN_TN8(1, 1, 8)
   MPNN_TN8(1, 2, 4)
 #undef MPNN_TN8
-  return false;
+  return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: no kernel for M=%d K=%d", a.M, a.K);
 }
 
 }  // namespace
@@ -378,6 +420,7 @@ extern "C" {
 
 int64_t mpnn_gemm_tn8_scratch_floats(int64_t N, int32_t M, int32_t K, int32_t K2, int32_t dtype) {
   if (N < 0 || M < 1 || K < 1 || K2 < 0) return -1;
+  if (N < kTn8Rows) return 0;
   return (int64_t)tn8_plan(N, M, K, K2, dtype == MPNN_BF16).blocks * M * ((int64_t)K + K2);
 }
 
@@ -390,10 +433,11 @@ int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bit
   if (N < 0 || M < 1 || K < 1 || K2 < 0 || M > kTn8MaxLd || K > kTn8MaxLd || K2 > kTn8MaxLd)
     return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: N=%lld M=%d K=%d K2=%d", (long long)N, M, K, K2);
   const int64_t ktot = (int64_t)K + K2;
+  if (M * ktot > (1 << 30)) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: M=%d x %lld outputs", M, (long long)ktot);
   if (!dW || lddw < ktot) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: dW is null or lddw below K + K2");
   const Tn8Plan p = tn8_plan(N, M, K, K2, bf16);
   if (N > 0) {
-    if (!G || !Q || !scale || !scratch || (K2 > 0 && (!Q2 || !scale2))) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: null pointer argument");
+    if (!G || !Q || !scale || (N >= kTn8Rows && !scratch) || (K2 > 0 && (!Q2 || !scale2))) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: null pointer argument");
     if (ldg < M || ldq < (K + 15) / 16 * 16 || (K2 > 0 && ldq2 < (K2 + 15) / 16 * 16) || (Gout && ldgo < M))
       return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: leading dimension too small");
     if (ldg > kTn8MaxLd || ldq > kTn8MaxLd || ldq2 > kTn8MaxLd || ldgo > kTn8MaxLd)
@@ -413,9 +457,16 @@ int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bit
     a.gout = Gout; a.ldgo = ldgo; a.partial = scratch; a.N = N; a.M = M;
     a.ktiles = p.ktiles;
     a.slabs = (int)((N + p.slab_rows - 1) / p.slab_rows);
-    const bool known = bf16 ? launch_tn8<bf16_t>(a, p, stream) : launch_tn8<float>(a, p, stream);
-    if (!known) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: no kernel for M=%d K=%d", M, K);
-    MPNN_LAUNCH_CHECK("k_gemm_tn8");
+    if (N < kTn8Rows) {
+      if ((M + 3) / 4 > 65535) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: M=%d", M);
+      const dim3 grid((unsigned)((ktot + 63) / 64), (unsigned)((M + 3) / 4));
+      if (bf16) k_gemm_tn8_few<bf16_t><<<grid, kBlock, 0, stream>>>(a, static_cast<bf16_t*>(dW), lddw);
+      else k_gemm_tn8_few<float><<<grid, kBlock, 0, stream>>>(a, static_cast<float*>(dW), lddw);
+      MPNN_LAUNCH_CHECK("k_gemm_tn8_few");
+      return MPNN_OK;
+    }
+    const int32_t rc = bf16 ? launch_tn8<bf16_t>(a, p, stream) : launch_tn8<float>(a, p, stream);
+    if (rc != MPNN_OK) return rc;
   }
   const int64_t count = (int64_t)M * ktot;
   const int64_t grid = (count + 63) / 64;

@@ -470,19 +470,20 @@ def test_entry_points_refuse_before_any_launch():
     b = lambda **k: lib.mpnn_relu_bits(*{**dict(y=p, ld=16, dt=0, n=4, m=16, b=p, st=None), **k}.values())
     for bad in (dict(dt=3), dict(n=-1), dict(m=0), dict(ld=15), dict(y=None), dict(b=None)):
         assert b(**bad) == -1, bad
-    base = dict(x=p, ldx=16, xd=0, xs=None, w=p, ldw=16, ws=p, bias=None, y=p, ldy=8, yd=0, n=4, k=16, m=8, relu=0, space=p, st=None)
+    base = dict(x=p, ldx=608, xd=0, xs=None, w=p, ldw=608, ws=p, bias=None, y=p, ldy=8, yd=0, n=4, k=600, m=8, relu=0, space=p, st=None)
     li = lambda **k: lib.mpnn_linear_int8(*{**base, **k}.values())
-    for bad in (dict(xd=2), dict(yd=3), dict(n=-1), dict(k=0), dict(k=8193), dict(m=0), dict(ldx=15), dict(ldw=8), dict(ldy=7),
-                dict(x=None), dict(w=None), dict(ws=None), dict(y=None), dict(space=None), dict(xd=3), dict(w=p + 4), dict(ldw=24),
-                dict(xd=3, xs=p, ldx=24), dict(xd=3, xs=p, x=p + 1), dict(space=p + 4)):
+    for bad in (dict(xd=2), dict(yd=3), dict(n=-1), dict(k=0), dict(k=8193), dict(m=0), dict(ldx=599), dict(ldw=600), dict(ldy=7),
+                dict(x=None), dict(w=None), dict(ws=None), dict(y=None), dict(space=None), dict(xd=3), dict(w=p + 4), dict(ldw=612),
+                dict(xd=3, xs=p, ldx=612), dict(xd=3, xs=p, x=p + 1), dict(space=p + 4)):
         assert li(**bad) == -1, bad
     assert li(n=0) == 0
-    assert lib.mpnn_linear_int8_workspace_bytes(-1, 1, 1, 0) == -1 and lib.mpnn_linear_int8_workspace_bytes(4, 16, 8, 3) == 0
+    assert lib.mpnn_linear_int8_workspace_bytes(-1, 1, 1, 0) == -1 and lib.mpnn_linear_int8_workspace_bytes(4, 600, 8, 3) == 0
+    assert lib.mpnn_linear_int8_workspace_bytes(4, 600, 8, 0) == 4 * 608 + 16 and lib.mpnn_linear_int8_workspace_bytes(4, 16, 8, 0) == 0
     base_t = dict(g=p, ldg=8, dt=0, bits=None, q=p, ldq=16, s=p, k=16, q2=None, ldq2=0, s2=None, k2=0, dw=p, lddw=16, scratch=p,
                   go=None, ldgo=0, n=4, m=8, st=None)
     tn = lambda **k: lib.mpnn_gemm_tn8(*{**base_t, **k}.values())
     for bad in (dict(dt=2), dict(n=-1), dict(m=0), dict(k=0), dict(k2=-1), dict(dw=None), dict(lddw=15), dict(g=None), dict(q=None),
-                dict(s=None), dict(scratch=None), dict(k2=4, lddw=20), dict(ldg=7), dict(ldq=8), dict(go=p, ldgo=7), dict(ldg=1 << 22),
+                dict(s=None), dict(n=128, scratch=None), dict(k2=4, lddw=20), dict(ldg=7), dict(ldq=8), dict(go=p, ldgo=7), dict(ldg=1 << 22),
                 dict(q=p + 2), dict(ldq=18), dict(dt=1, ldg=9), dict(dt=1, m=7), dict(dt=1, g=p + 2)):
         assert tn(**bad) == -1, bad
     assert lib.mpnn_gemm_tn8_scratch_floats(-1, 8, 8, 0, 0) == -1
