@@ -17,12 +17,11 @@
 //           KiB per step of 128 and CU, three quarters of the matrix cores' time) and, for short K, the results.
 //   thin    few rows: a wave per 32 x 32 outputs, operands from memory as they lie.  Bound by latency.
 #include "common.h"
-#include "rowio.h"
+#include "rows8.h"
 
 namespace mpnn {
 namespace {
 
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kI8MaxK = 8192;
@@ -55,68 +54,6 @@ __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int left) {
   }
   return v;
 }
-
-// V consecutive outputs of a row.
-template <typename Y, int V>
-__device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int left, bool wide) {
-  if (wide && left >= V) {
-    if constexpr (sizeof(Y) == 4) {
-#pragma unroll
-      for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-      uint32_t w[V / 2];
-#pragma unroll
-      for (int j = 0; j < V; j += 2) w[j / 2] = pack_bf16(v[j], v[j + 1]);
-      if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-      else
-#pragma unroll
-        for (int j = 0; j < V / 2; j += 4) *reinterpret_cast<uint4*>(p + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < left) p[j] = f32_to_scalar<Y>(v[j]);
-  }
-}
-
-// Results of a wave on their way to memory: ROWS rows x 64 outputs in LDS, from where whole row segments leave (128 bytes
-// in bfloat16, 256 in float32; stores of 64 bytes per row took 1.65 instead of 1.20 ms for 4 M rows of 256 in float32).
-// 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread.  Only
-// the wave that owns the patch touches it.
-template <typename Y, int ROWS>
-struct Patch {
-  static constexpr int VEC = 16 / sizeof(Y), CHUNKS = 64 / VEC, BYTES = ROWS * 64 * sizeof(Y);
-  char* base;
-  __device__ __forceinline__ void put(int row, int chunk, const float (&v)[VEC]) const {
-    store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (64 * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
-  }
-  // Rows r0 .. of the matrix, outputs m .. m + 63 of which those below `end` exist.
-  __device__ __forceinline__ void leave(const I8Args& a, int64_t r0, int m, int end) const {
-    const int lane = threadIdx.x & 63;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int q = 0; q < ROWS * CHUNKS / 64; ++q) {
-      const int r = q * (64 / CHUNKS) + lane / CHUNKS, chunk = lane % CHUNKS;
-      const i32x4 v = *reinterpret_cast<const i32x4*>(base + r * (64 * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
-      const int left = end - m - chunk * VEC;
-      if (r0 + r >= a.N || left <= 0) continue;
-      Y* const y = static_cast<Y*>(a.y) + (r0 + r) * a.ldy + m + chunk * VEC;
-      if (a.wide_out && left >= VEC) {
-        __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(y));   // nobody reads them here: the L2 keeps x and the weights
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (e < left) {
-            if constexpr (sizeof(Y) == 4) y[e] = __uint_as_float((uint32_t)v[e]);
-            else y[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
-          }
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-};
 
 // ------------------------------------------------------------------------------------------------------------- rows
 // A wave owns 16 rows at a time.  Lane (row i = lane % 16, group g = lane / 16) holds 16 values of every step of 64
@@ -264,10 +201,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
           float v[16];
           values_of<X>(raw[s], s, g, a.K, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
-            top = m > top ? m : top;
-          }
+          for (int e = 0; e < 16; ++e) top = magnitude_bits(v[e]) > top ? magnitude_bits(v[e]) : top;
         }
       {   // the row's other three groups
         uint32_t o = __shfl_xor(top, 16, 64);
@@ -275,24 +209,15 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
         o = __shfl_xor(top, 32, 64);
         top = o > top ? o : top;
       }
-      const bool finite = top < 0x7f800000u, zero = __uint_as_float(top) < 0x1p-100f;
-      const float inv = (zero || !finite) ? 0.f : 127.f / __uint_as_float(top);
-      xs = !finite ? __builtin_nanf("") : (zero ? 0.f : __uint_as_float(top) / 127.f);
-      const uint32_t keep = finite ? ~0u : 0u;
+      const Quant qt = quant_of(top);
+      xs = qt.scale;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
         if (s < steps) {
           float v[16];
           values_of<X>(raw[s], s, g, a.K, v);
-          uint32_t b[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) b[e] = __float_as_uint(fmaf(v[e], inv, 12582912.f));   // rows8.hip: whole numbers in the last place
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = __builtin_amdgcn_perm(b[4 * j + 1], b[4 * j], 0x0c0c0400u);
-            const uint32_t hi = __builtin_amdgcn_perm(b[4 * j + 3], b[4 * j + 2], 0x04000c0cu);
-            q[s][j] = (int32_t)((lo | hi) & keep);
-          }
+          for (int j = 0; j < 4; ++j) q[s][j] = (int32_t)quant_word(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], qt);
         }
     }
     if (tile + step < tiles) fetch(tile + step);
@@ -322,7 +247,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
       } else {
         patch.put(i, chunk, v);
       }
-      if ((b & 32) || b + 32 >= m_pad) patch.leave(a, 16 * tile, m_begin + (b & ~63), m_begin + m_count);
+      if ((b & 32) || b + 32 >= m_pad) patch.leave(a.y, a.ldy, a.N, 16 * tile, m_begin + (b & ~63), m_begin + m_count, a.wide_out);
     }
   }
 }
@@ -523,7 +448,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
         }
         patch.put(i32, half * (32 / VEC) + c, v);
       }
-      patch.leave(a, n0 + (wn * TN + j) * 32, mw, a.M);
+      patch.leave(a.y, a.ldy, a.N, n0 + (wn * TN + j) * 32, mw, a.M, a.wide_out);
     }
   }
 }

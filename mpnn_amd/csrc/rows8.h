@@ -1,0 +1,95 @@
+// Device-side pieces shared by the kernels around 8-bit rows (rows8.hip holds the format's definition).
+#pragma once
+#include "rowio.h"
+
+namespace mpnn {
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+// What a row's largest magnitude (as the bits of a float: infinities and NaN compare above every finite one) makes of it.
+struct Quant {
+  float inv, scale;
+  uint32_t keep;   // all ones, or zeros for a row that is not finite
+};
+__device__ __forceinline__ Quant quant_of(uint32_t top) {
+  const float t = __uint_as_float(top);
+  const bool finite = top < 0x7f800000u, zero = t < 0x1p-100f;
+  Quant r;
+  r.inv = (zero || !finite) ? 0.f : 127.f / t;
+  r.scale = !finite ? __builtin_nanf("") : (zero ? 0.f : t / 127.f);
+  r.keep = finite ? ~0u : 0u;
+  return r;
+}
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// The byte of v: 1.5 * 2^23 added in the same rounding leaves the whole number in the low byte.
+__device__ __forceinline__ uint32_t quant_bits(float v, float inv) { return __float_as_uint(fmaf(v, inv, 12582912.f)); }
+__device__ __forceinline__ uint32_t quant_word(float a, float b, float c, float d, const Quant& q) {
+  const uint32_t lo = __builtin_amdgcn_perm(quant_bits(b, q.inv), quant_bits(a, q.inv), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(quant_bits(d, q.inv), quant_bits(c, q.inv), 0x04000c0cu);
+  return (lo | hi) & q.keep;
+}
+
+// V consecutive outputs of a row; `left` of them exist.
+template <typename Y, int V>
+__device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int left, bool wide) {
+  if (wide && left >= V) {
+    if constexpr (sizeof(Y) == 4) {
+#pragma unroll
+      for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+      uint32_t w[V / 2];
+#pragma unroll
+      for (int j = 0; j < V; j += 2) w[j / 2] = pack_bf16(v[j], v[j + 1]);
+      if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      else
+#pragma unroll
+        for (int j = 0; j < V / 2; j += 4) *reinterpret_cast<uint4*>(p + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < left) p[j] = f32_to_scalar<Y>(v[j]);
+  }
+}
+
+// Results of a wave on their way to memory: ROWS rows x 64 outputs in LDS, from where whole row segments leave (128 bytes
+// in bfloat16, 256 in float32; stores of 64 bytes per row took 1.65 instead of 1.20 ms for 4 M rows of 256 in float32).
+// 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread.  Only
+// the wave that owns the patch touches it.
+template <typename Y, int ROWS>
+struct Patch {
+  static constexpr int VEC = 16 / sizeof(Y), CHUNKS = 64 / VEC, BYTES = ROWS * 64 * sizeof(Y);
+  char* base;
+  __device__ __forceinline__ void put(int row, int chunk, const float (&v)[VEC]) const {
+    store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (64 * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
+  }
+  // To rows r0 .. of y [N, ldy], outputs m .. m + 63 of which those below `end` exist; wide: 16-byte stores are possible.
+  __device__ __forceinline__ void leave(void* y, int64_t ldy, int64_t N, int64_t r0, int m, int end, bool wide) const {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < ROWS * CHUNKS / 64; ++q) {
+      const int r = q * (64 / CHUNKS) + lane / CHUNKS, chunk = lane % CHUNKS;
+      const i32x4 v = *reinterpret_cast<const i32x4*>(base + r * (64 * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
+      const int left = end - m - chunk * VEC;
+      if (r0 + r >= N || left <= 0) continue;
+      Y* const p = static_cast<Y*>(y) + (r0 + r) * ldy + m + chunk * VEC;
+      if (wide && left >= VEC) {
+        __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(p));   // not read here again: the L2 keeps the operands
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (e < left) {
+            if constexpr (sizeof(Y) == 4) p[e] = __uint_as_float((uint32_t)v[e]);
+            else p[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
+          }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+}  // namespace mpnn

@@ -12,30 +12,12 @@
 // Bound: memory, one pass: a row is read once into the registers of LPR lanes, its top found by shuffles, and its bytes
 // written from there.
 #include "common.h"
-#include "rowio.h"
+#include "rows8.h"
 
 namespace mpnn {
 namespace {
 
 constexpr int kRows8MaxK = 8192;
-
-struct Quant {
-  float inv, scale;
-};
-
-__device__ __forceinline__ Quant quant_of(float top, bool finite) {
-  Quant r;
-  const bool zero = top < 0x1p-100f;
-  r.inv = (zero || !finite) ? 0.f : 127.f / top;
-  r.scale = !finite ? __builtin_nanf("") : (zero ? 0.f : top / 127.f);
-  return r;
-}
-
-// The byte of x * inv.  inv = 0 (rows of zeros, rows that are not finite): 0 whatever x is.
-__device__ __forceinline__ uint32_t quant_byte(float x, float inv) {
-  const float r = fmaf(x, inv, 12582912.f);   // 1.5 * 2^23
-  return inv == 0.f ? 0u : (__float_as_uint(r) & 0xffu);
-}
 
 struct QuantArgs {
   const void* x;
@@ -68,10 +50,7 @@ __global__ void __launch_bounds__(kBlock) k_quantize_rows(QuantArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const uint32_t m = __float_as_uint(v[i][k]) & 0x7fffffffu;
-        top = m > top ? m : top;
-      }
+      for (int k = 0; k < VEC; ++k) top = magnitude_bits(v[i][k]) > top ? magnitude_bits(v[i][k]) : top;
     constexpr int W = LPR < 64 ? LPR : 64;
 #pragma unroll
     for (int off = W / 2; off > 0; off >>= 1) {
@@ -84,20 +63,19 @@ __global__ void __launch_bounds__(kBlock) k_quantize_rows(QuantArgs a) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) top = red[turn][w] > top ? red[turn][w] : top;
     }
-    const Quant qt = quant_of(__uint_as_float(top), top < 0x7f800000u);
+    const Quant qt = quant_of(top);
     int8_t* q = a.q + row * a.ldq;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LPR + lane) * VEC;
       if (c >= a.Kp) continue;
       if constexpr (VEC == 1) {
-        q[c] = (int8_t)quant_byte(v[i][0], qt.inv);
+        q[c] = (int8_t)(quant_bits(v[i][0], qt.inv) & qt.keep);
       } else {
         uint32_t w[VEC / 4];
 #pragma unroll
         for (int k = 0; k < VEC; k += 4)
-          w[k / 4] = quant_byte(v[i][k], qt.inv) | quant_byte(v[i][k + 1], qt.inv) << 8 |
-                     quant_byte(v[i][k + 2], qt.inv) << 16 | quant_byte(v[i][k + 3], qt.inv) << 24;
+          w[k / 4] = quant_word(v[i][k], v[i][k + 1], v[i][k + 2], v[i][k + 3], qt);
         if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(q + c) = w[0];
         else *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
       }

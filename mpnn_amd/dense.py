@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import Rows8, gemm_tn8, quantize_rows, relu_bits
+from .rows8 import Rows8, gemm_tn8, kept_linear, quantize_rows, relu_bits
 
 _SCRATCH = {}
 
@@ -238,12 +238,15 @@ class _ProjectKept(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, rows):
+        y = None
+        if ctx.needs_input_grad[1] and rows is None:
+            both = kept_linear(x, w) if x.dtype == torch.bfloat16 else None      # one pass over x
+            y, rows = (both[0], both[1]) if both is not None else (None, quantize_rows(x))
         if ctx.needs_input_grad[1]:
-            rows = quantize_rows(x) if rows is None else rows
             ctx.save_for_backward(w, rows.values, rows.scale)
         else:
             ctx.save_for_backward(w, None, None)
-        return _kit(x.dtype)[0](x, w)
+        return _kit(x.dtype)[0](x, w) if y is None else y
 
     @staticmethod
     @once_differentiable
@@ -261,16 +264,20 @@ class _UpdateKept(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, aggr, w_out):
         f = x.size(1)
-        wx, wa = w_out[:, :f], w_out[:, f:]
-        if x.dtype == torch.bfloat16:
-            wx, wa = wx.contiguous(), wa.contiguous()
-        y = _kit(x.dtype)[0](x, wx, aggr, wa, relu=True)
-        kept = (None,) * 4
-        if ctx.needs_input_grad[2]:
-            rx, ra = quantize_rows(x), quantize_rows(aggr)
-            kept = (rx.values, rx.scale, ra.values, ra.scale)
         ctx.f = f
-        ctx.save_for_backward(w_out, relu_bits(y), *kept)
+        bf = x.dtype == torch.bfloat16
+        if bf and not bf16_ok(w_out):
+            w_out = w_out.contiguous()
+        want = ctx.needs_input_grad[2]
+        both = kept_linear(x, w_out, aggr, relu=True) if bf and want else None   # one pass over x and aggr
+        if both is not None:
+            y, rx, ra, bits = both
+        else:
+            y = _kit(x.dtype)[0](x, w_out[:, :f], aggr, w_out[:, f:], relu=True)
+            rx, ra = (quantize_rows(x), quantize_rows(aggr)) if want else (None, None)
+            bits = relu_bits(y)
+        kept = (rx.values, rx.scale, ra.values, ra.scale) if want else (None,) * 4
+        ctx.save_for_backward(w_out, bits, *kept)
         return y
 
     @staticmethod
@@ -288,8 +295,13 @@ class _UpdateKept(torch.autograd.Function):
         if need[0] or need[1]:
             nt = _kit(gy.dtype)[0]
             wt = w_out.t().contiguous()
-            gx = nt(gz, wt[:f]) if need[0] else None
-            ga = nt(gz, wt[f:]) if need[1] else None
+            if need[0] and need[1]:
+                g_both = nt(gz, wt)              # one pass over gz: the two gradients are column halves of it
+                gx, ga = g_both[:, :f], g_both[:, f:]
+            elif need[0]:
+                gx = nt(gz, wt[:f])
+            else:
+                ga = nt(gz, wt[f:])
         return gx, ga, gw
 
 

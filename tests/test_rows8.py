@@ -321,41 +321,91 @@ def test_gemm_tn8_strides_no_rows_and_rows_that_are_not_finite():
 # ----------------------------------------------------------------------------------------------- the dense products
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_project_and_update_keep_their_inputs_in_8_bits(dtype):
+@pytest.mark.parametrize("n,f,h", [(777, 40, 24), (1, 8, 8), (130, 128, 128), (500, 64, 64), (300, 264, 32), (50, 16, 256), (129, 96, 200)])
+def test_project_and_update_keep_their_inputs_in_8_bits(n, f, h, dtype):
+    """Against 64 bits with the 8-bit rows in the weight gradient's place of the inputs.  Sums of c float32 terms in some
+    order: 2 c u times the magnitudes (float32 inputs are cut into three pieces: 3 c terms); bfloat16 gradients of the
+    update carry one rounding of g * open, which is exact."""
     from mpnn_amd import quantize_rows
     from mpnn_amd.dense import project, update
-    n, f, h = 777, 40, 24
     leaf = lambda *s, seed: randn(*s, seed=seed, dtype=dtype).cuda().requires_grad_()
     x, a, w, wo = leaf(n, f, seed=1), leaf(n, h, seed=2), leaf(2 * h, f, seed=3), leaf(h, f + h, seed=4)
     gy, gy2 = randn(n, 2 * h, seed=5, dtype=dtype).cuda(), randn(n, h, seed=6, dtype=dtype).cuda()
+    d = lambda t: t.detach().double().cpu()
+    deq = lambda t: d(quantize_rows(t.detach()).values) * d(quantize_rows(t.detach()).scale).unsqueeze(1)
 
-    def deviation(g, *xs):
-        """How far a weight gradient may be off for its inputs being off by half a step (and both being rounded)."""
-        s = [quantize_rows(t.detach()).scale.double().unsqueeze(1).expand(-1, t.size(1)) for t in xs]
-        return g.double().abs().t() @ torch.cat(s, dim=1) * (0.5 + 1e-3)
+    def product(p, q):
+        """p @ q and the bound of its error."""
+        return p @ q, 2 * 3 * (p.size(1) + 80) * U * (p.abs() @ q.abs()) + 2.0 ** -16 * (0 if dtype == torch.float32 else 1) * (p.abs() @ q.abs())
 
-    plain, kept = project(x, w), project(x, w, checkpoint="int8")
-    assert torch.equal(plain, kept)
-    (px, pw), (kx, kw) = torch.autograd.grad(plain, (x, w), gy), torch.autograd.grad(kept, (x, w), gy)
-    assert torch.equal(px, kx)
-    assert ((pw - kw).double().abs() <= deviation(gy, x) + 2 * torch.finfo(dtype).eps * pw.double().abs()).all()
+    kept = project(x, w, checkpoint="int8")
+    gx, gw = torch.autograd.grad(kept, (x, w), gy)
+    close(kept, *product(d(x), d(w).t()))
+    close(gx, *product(d(gy), d(w)))
+    close(gw, *product(d(gy).t(), deq(x)))
     brought = project(x, w, checkpoint=quantize_rows(x))
-    assert torch.equal(torch.autograd.grad(brought, w, gy)[0], kw)
-    plain, kept = update(x, a, wo), update(x, a, wo, checkpoint="int8")
-    assert torch.equal(plain, kept)
-    p, k = torch.autograd.grad(plain, (x, a, wo), gy2), torch.autograd.grad(kept, (x, a, wo), gy2)
-    assert torch.equal(p[0], k[0]) and torch.equal(p[1], k[1])
-    gz = gy2 * (plain > 0)
-    assert ((p[2] - k[2]).double().abs() <= deviation(gz, x, a) + 2 * torch.finfo(dtype).eps * p[2].double().abs()).all()
-    # with and without each gradient
-    kept = update(x.detach(), a, wo.detach(), checkpoint="int8")
-    assert torch.equal(torch.autograd.grad(kept, a, gy2)[0], p[1])
-    kept = update(x.detach(), a.detach(), wo, checkpoint="int8")
-    assert torch.equal(torch.autograd.grad(kept, wo, gy2)[0], k[2])
-    assert torch.equal(torch.autograd.grad(project(x, w.detach(), checkpoint="int8"), x, gy)[0], px)
+    assert torch.equal(torch.autograd.grad(brought, w, gy)[0], gw)
+    assert torch.equal(torch.autograd.grad(project(x, w.detach(), checkpoint="int8"), x, gy)[0], gx)
     (g,) = torch.autograd.grad(project(x, w, checkpoint="int8").sum(), w)       # an expanded upstream gradient
-    ones = torch.ones_like(gy)
-    assert torch.equal(g, torch.autograd.grad(project(x, w, checkpoint="int8"), w, ones)[0])
+    assert torch.equal(g, torch.autograd.grad(project(x, w, checkpoint="int8"), w, torch.ones_like(gy))[0])
+
+    kept = update(x, a, wo, checkpoint="int8")
+    both = torch.cat([d(x), d(a)], dim=1)
+    z, bound = product(both, d(wo).t())
+    close(kept, z.clamp_min(0), bound)
+    gz = d(gy2) * (d(kept) > 0)
+    gx, ga, gw = torch.autograd.grad(kept, (x, a, wo), gy2)
+    g_in, bound = product(gz, d(wo))
+    close(gx, g_in[:, :f], bound[:, :f])
+    close(ga, g_in[:, f:], bound[:, f:])
+    close(gw, *product(gz.t(), torch.cat([deq(x), deq(a)], dim=1)))
+    # with and without each gradient
+    for needs in ((0, 1, 0), (1, 0, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1), (1, 1, 0)):
+        ins = [t if k else t.detach() for t, k in zip((x, a, wo), needs)]
+        part = torch.autograd.grad(update(*ins, checkpoint="int8"), [t for t, k in zip(ins, needs) if k], gy2)
+        full = [t for t, k in zip((gx, ga, gw), needs) if k]
+        for p, q, k in zip(part, full, [k for k in range(3) if needs[k]]):
+            # the forward without a weight gradient may add in another order: its relu is the same unless z is zero to rounding
+            if needs[2]:
+                assert torch.equal(p, q) or k < 2
+            close(p, d(q), 2 * bound.max() + torch.finfo(dtype).eps * d(q).abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,k2,m", [(1, 8, 0, 8), (15, 32, 0, 40), (16, 40, 8, 32), (17, 64, 64, 64), (100, 128, 128, 128),
+                                      (129, 256, 0, 64), (300, 256, 256, 56), (1000, 128, 0, 256), (3001, 72, 136, 104), (40000, 128, 128, 128)])
+@pytest.mark.parametrize("relu", [False, True])
+def test_kept_linear_leaves_what_the_separate_passes_do(n, k, k2, m, relu):
+    from mpnn_amd.rows8 import kept_linear, quantize_rows, relu_bits
+    x = randn(n, k, seed=n, dtype=torch.bfloat16).cuda()
+    x2 = randn(n, k2, seed=n + 1, dtype=torch.bfloat16).cuda() if k2 else None
+    w = randn(m, k + k2, seed=n + 2, dtype=torch.bfloat16).cuda()
+    if n > 20:
+        x[3] = 0
+        x[5, 2] = float("inf")
+        x[n - 1, k - 1] = float("nan")
+    y, r, r2, bits = kept_linear(x, w, x2, relu=relu)
+    for rows, t in ((r, x), (r2, x2)):
+        if t is not None:
+            q = quantize_rows(t)
+            assert torch.equal(rows.values, q.values) and torch.equal(rows.scale.nan_to_num(nan=-1), q.scale.nan_to_num(nan=-1))
+            assert torch.equal(torch.as_strided(rows.values, (n, rows.pitch), (rows.pitch, 1)), torch.as_strided(q.values, (n, q.pitch), (q.pitch, 1)))
+    both = torch.cat([x] + ([x2] if k2 else []), dim=1).double()
+    fine = torch.isfinite(both).all(dim=1)
+    want = both[fine] @ w.double().t()
+    size = both[fine].abs() @ w.double().abs().t()
+    want = want.clamp_min(0) if relu else want
+    bound = 2 * (k + k2) * U * size
+    got = y[fine].double()
+    assert bool(((got - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all())
+    if relu:
+        assert torch.equal(bits, relu_bits(y))
+    else:
+        assert bits is None
+    if n > 20:
+        assert not torch.isfinite(y[5]).all()
+        assert y[n - 1].isnan().all()
+        assert kept_linear(x.t().contiguous().t(), w, x2) is None          # rows that cannot be read in place
 
 
 @pytest.mark.gpu
