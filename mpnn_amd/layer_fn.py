@@ -25,9 +25,13 @@ from __future__ import annotations
 
 import torch
 
+from torch.autograd.function import once_differentiable
+
 from . import islands, ops
 from .dense import gemm_nt, gemm_nt_bf16, gemm_tn, gemm_tn_bf16
 from .graph import MPGraph
+from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
+from .rows8 import Rows8, gemm_tn8, kept_linear, quantize_rows, relu_bits
 
 
 def fused_x(dtype, f: int, h: int) -> bool:
@@ -184,6 +188,60 @@ class _LayerFn(torch.autograd.Function):
         return gx, None, g_wn, g_we, g_wout, None
 
 
+class _KeptLayerFn(torch.autograd.Function):
+    """The layer with its inputs held in 8 bits between the passes (rows8.py): x and aggr as 8-bit rows, the relu of the
+    update in one bit per entry, the projection not at all where the edge pass left its own relu bits.  Per node of width
+    H in float32: 2 H + H / 8 bytes and the edge pass's counts and bits instead of 16 H bytes more.  Same calls as
+    _LayerFn's general path otherwise; the weight gradients take the values that the 8-bit rows stand for."""
+
+    @staticmethod
+    def forward(ctx, x, edge_attr, w_nodes, w_edge, w_out, graph: MPGraph):
+        bf = x.dtype == torch.bfloat16
+        f, h = x.size(1), w_out.size(0)
+        w_edge, w_out = w_edge.contiguous(), w_out.contiguous()
+        ab = gemm_nt_bf16(x, w_nodes.contiguous()) if bf else gemm_nt(x, w_nodes)
+        a, b = ab[:, :h], ab[:, h:]
+        ea_s, ea_t = ops._prepare(a, b, edge_attr, w_edge, graph)
+        aggr, cnt, maskbits = ops._run_forward(a, b, ea_s, w_edge, graph.by_dst, graph, True)
+        both = kept_linear(x, w_out, aggr, relu=True) if bf else None
+        if both is not None:
+            y, rx, ra, bits = both
+        else:
+            y = (gemm_nt_bf16 if bf else gemm_nt)(x, w_out[:, :f], aggr, w_out[:, f:], relu=True)
+            rx, ra, bits = quantize_rows(x), quantize_rows(aggr), relu_bits(y)
+        if maskbits is not None:
+            graph.tpos                       # built once per graph, outside the backward
+        ctx.save_for_backward(rx.values, rx.scale, ra.values, ra.scale, bits, cnt[0], cnt[1], maskbits,
+                              ab if maskbits is None else None, ea_t, w_nodes, w_edge, w_out)
+        ctx.graph = graph
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        xv, xs, av, as_, bits, cnt8, cnt_big, maskbits, ab, ea_t, w_nodes, w_edge, w_out = ctx.saved_tensors
+        graph = ctx.graph
+        bf = gy.dtype == torch.bfloat16
+        nt = gemm_nt_bf16 if bf else gemm_nt
+        f, h = xv.size(1), w_out.size(0)
+        rx, n = Rows8(xv, xs), xv.size(0)
+        gy = gy.contiguous()
+        if gy.data_ptr() % 16:
+            gy = gy.clone()
+        gz = torch.empty_like(gy)
+        g_wout = gemm_tn8(gy, rx, Rows8(av, as_), bits=bits, g_out=gz)
+        wt_out = w_out.t().contiguous()                   # [F+H, H]
+        g_ab = torch.empty((n, 2 * h), dtype=gy.dtype, device=gy.device)
+        cnt = (cnt8, cnt_big)
+        ga = nt(gz, wt_out[f:], emul=cnt8, out2=g_ab[:, :h])
+        ops.count_fixup(ga, cnt, graph.by_dst, g_ab[:, :h])
+        a, b = (ab[:, :h], ab[:, h:]) if ab is not None else (ga, ga)     # not read where the edge pass left bits
+        g_we = ops._run_backward_src(a, b, ga, ea_t, w_edge, graph.by_src, graph, g_ab[:, h:], maskbits)
+        gx = nt(gz, wt_out[:f], g_ab, w_nodes.t().contiguous()) if ctx.needs_input_grad[0] else None
+        g_wn = gemm_tn8(g_ab, rx) if ctx.needs_input_grad[2] else None
+        return gx, None, g_wn, g_we if ctx.needs_input_grad[3] else None, g_wout if ctx.needs_input_grad[4] else None, None
+
+
 class _EgnnLayerFn(torch.autograd.Function):
     """EGNN layer (message pass + coordinate update in one edge pass, then the update) as one node, float32 or
     bfloat16 storage, every product on the library's MFMA kernels:
@@ -307,6 +365,23 @@ def layer_forward_eager(x, edge_attr, w_nodes, w_edge, w_out, graph: MPGraph) ->
     if x.dtype == torch.bfloat16 and islands.plan_for(graph, x.size(1), w_out.size(0), edge_attr.size(1), False) is None:
         x, w_nodes, w_out = _pad_features(x, w_nodes, w_out)     # (the one-launch kernels take any input width)
     return _LayerFn.apply(x, edge_attr, w_nodes, w_edge, w_out, graph)
+
+
+@torch.compiler.disable
+def kept_layer_forward(x, edge_attr, w_nodes, w_edge, w_out, graph: MPGraph) -> torch.Tensor:
+    """layer_forward with the layer's inputs held in 8 bits until its backward.  Graphs whose layer is one launch (batches
+    of molecules and point clouds) keep little beyond x already and run as they do."""
+    _check_dtypes(x, edge_attr, w_nodes, w_edge, w_out)
+    if (islands.plan_for(graph, x.size(1), w_out.size(0), edge_attr.size(1), False) is not None
+            or not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_nodes, w_edge, w_out)))):
+        return layer_forward_eager(x, edge_attr, w_nodes, w_edge, w_out, graph)
+    if max(x.size(1), w_out.size(0)) > ROWS8_MAX_WIDTH:
+        raise ValueError(f"8-bit rows are at most {ROWS8_MAX_WIDTH} wide, got {tuple(x.shape)} and {tuple(w_out.shape)}")
+    if x.dtype == torch.bfloat16:
+        x, w_nodes, w_out = _pad_features(x, w_nodes, w_out)
+    elif not x.is_contiguous():
+        x = x.contiguous()
+    return _KeptLayerFn.apply(x, edge_attr, w_nodes, w_edge, w_out, graph)
 
 
 def egnn_layer_forward_eager(x, pos, edge_attr, w_nodes, w_edge, w_out, w_pos, graph: MPGraph):

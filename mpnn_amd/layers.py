@@ -43,9 +43,18 @@ class _SplitCatWeight(torch.autograd.Function):
         return g, None
 
 
+def _checkpoint(checkpoint):
+    if checkpoint not in (None, "int8"):
+        raise ValueError(f'checkpoint must be None or "int8", got {checkpoint!r}')
+    return checkpoint
+
+
 class MPNNLayerCat(torch.nn.Module):
-    def __init__(self, in_channels, edge_channels, out_channels):
+    """``checkpoint="int8"`` (no counterpart in the reference): what the layer keeps for its backward waits in 8 bits."""
+
+    def __init__(self, in_channels, edge_channels, out_channels, checkpoint=None):
         super().__init__()
+        self.checkpoint = _checkpoint(checkpoint)
         self.in_channels, self.edge_channels, self.out_channels = in_channels, edge_channels, out_channels
         self.linear = Linear((in_channels * 2) + edge_channels, out_channels, bias=False)
         self.linear_out = Linear(out_channels + in_channels, out_channels, bias=False)
@@ -53,6 +62,9 @@ class MPNNLayerCat(torch.nn.Module):
     def forward(self, x, edge_index, edge_attr):
         # [Wi ; Wj] stacked row-wise gives the [N, 2H] table (target half, source half) in one GEMM.
         w_nodes, w_edge = _SplitCatWeight.apply(self.linear.weight, self.in_channels)
+        if self.checkpoint:
+            return layer_fn.kept_layer_forward(x, edge_attr, w_nodes, w_edge, self.linear_out.weight,
+                                               graph_for(edge_index, x.size(0)))
         if torch.compiler.is_compiling():      # torch.compile(model), experiments/flickr_exp.py:30: one opaque operator
             return compiled_ops.layer(x, edge_index, edge_attr, w_nodes, w_edge, self.linear_out.weight)
         graph = graph_for_eager(edge_index, x.size(0))
@@ -60,8 +72,11 @@ class MPNNLayerCat(torch.nn.Module):
 
 
 class MPNNLayerSum(torch.nn.Module):
-    def __init__(self, in_channels, edge_channels, out_channels):
+    """``checkpoint="int8"`` (no counterpart in the reference): what the layer keeps for its backward waits in 8 bits."""
+
+    def __init__(self, in_channels, edge_channels, out_channels, checkpoint=None):
         super().__init__()
+        self.checkpoint = _checkpoint(checkpoint)
         self.in_channels, self.edge_channels, self.out_channels = in_channels, edge_channels, out_channels
         self.fused_linear = Linear(in_channels, out_channels * 2, bias=False)
         self.linear_3 = Linear(edge_channels, out_channels, bias=False)
@@ -69,6 +84,9 @@ class MPNNLayerSum(torch.nn.Module):
 
     def forward(self, x, edge_index, edge_attr):
         # xs = AB[:, :H] (target half), xt = AB[:, H:] (source half) of the fused projection
+        if self.checkpoint:
+            return layer_fn.kept_layer_forward(x, edge_attr, self.fused_linear.weight, self.linear_3.weight,
+                                               self.linear_out.weight, graph_for(edge_index, x.size(0)))
         if torch.compiler.is_compiling():      # torch.compile(model), experiments/flickr_exp.py:30: one opaque operator
             return compiled_ops.layer(x, edge_index, edge_attr, self.fused_linear.weight, self.linear_3.weight,
                                       self.linear_out.weight)

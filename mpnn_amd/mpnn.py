@@ -23,21 +23,23 @@ def _relu_after(layer, x):
     return x if isinstance(layer, (MPNNLayerCat, MPNNLayerSum)) else F.relu(x)
 
 
-def _make_layers(in_channels, edge_channels, hidden_channels, num_layers, mode):
+def _make_layers(in_channels, edge_channels, hidden_channels, num_layers, mode, checkpoint=None):
     cls = MPNNLayerCat if mode == 'cat' else MPNNLayerSum
     layers = torch.nn.ModuleList()
-    layers.append(cls(in_channels, edge_channels, hidden_channels))
+    layers.append(cls(in_channels, edge_channels, hidden_channels, checkpoint=checkpoint))
     for _ in range(num_layers - 1):
-        layers.append(cls(hidden_channels, edge_channels, hidden_channels))
+        layers.append(cls(hidden_channels, edge_channels, hidden_channels, checkpoint=checkpoint))
     return layers
 
 
 class MPNN(torch.nn.Module):
-    """Node-level model (Flickr); edge_channels is fixed to 4 as in the reference (models/mpnn.py:72-81)."""
+    """Node-level model (Flickr); edge_channels is fixed to 4 as in the reference (models/mpnn.py:72-81).
+    ``checkpoint="int8"`` (no counterpart there): the layers' inputs wait for the backward in 8 bits, which is what lets
+    deeper stacks of a large graph fit."""
 
-    def __init__(self, in_channels, hidden_channels, out_channels, num_layers=2, mode="cat"):
+    def __init__(self, in_channels, hidden_channels, out_channels, num_layers=2, mode="cat", checkpoint=None):
         super().__init__()
-        self.layers = _make_layers(in_channels, 4, hidden_channels, num_layers, mode)
+        self.layers = _make_layers(in_channels, 4, hidden_channels, num_layers, mode, checkpoint)
         self.output_layer = Linear(hidden_channels, out_channels)
 
     def forward(self, x, edge_index, edge_attr):
