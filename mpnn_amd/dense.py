@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import Rows8, gemm_tn8, kept_linear, quantize_rows, relu_bits
+from .rows8 import Rows8, gemm_tn8, kept_linear, relu_bits, rows8_of, to_rows8
 
 _SCRATCH = {}
 
@@ -241,7 +241,7 @@ class _ProjectKept(torch.autograd.Function):
         y = None
         if ctx.needs_input_grad[1] and rows is None:
             both = kept_linear(x, w) if x.dtype == torch.bfloat16 else None      # one pass over x
-            y, rows = (both[0], both[1]) if both is not None else (None, quantize_rows(x))
+            y, rows = (both[0], both[1]) if both is not None else (None, to_rows8(_lib.rows_in_place(x)))
         if ctx.needs_input_grad[1]:
             ctx.save_for_backward(w, rows.values, rows.scale)
         else:
@@ -254,7 +254,7 @@ class _ProjectKept(torch.autograd.Function):
         w, values, scale = ctx.saved_tensors
         g = _upstream(g)
         gx = _kit(g.dtype)[0](g, w.t().contiguous()) if ctx.needs_input_grad[0] else None
-        gw = gemm_tn8(g, Rows8(values, scale)) if ctx.needs_input_grad[1] else None
+        gw = gemm_tn8(g, rows8_of(values, scale)) if ctx.needs_input_grad[1] else None
         return gx, gw, None
 
 
@@ -274,7 +274,7 @@ class _UpdateKept(torch.autograd.Function):
             y, rx, ra, bits = both
         else:
             y = _kit(x.dtype)[0](x, w_out[:, :f], aggr, w_out[:, f:], relu=True)
-            rx, ra = (quantize_rows(x), quantize_rows(aggr)) if want else (None, None)
+            rx, ra = (to_rows8(_lib.rows_in_place(x)), to_rows8(_lib.rows_in_place(aggr))) if want else (None, None)
             bits = relu_bits(y)
         kept = (rx.values, rx.scale, ra.values, ra.scale) if want else (None,) * 4
         ctx.save_for_backward(w_out, bits, *kept)
@@ -289,7 +289,7 @@ class _UpdateKept(torch.autograd.Function):
         gz = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device) if need[0] or need[1] else None
         gx = ga = gw = None
         if need[2]:
-            gw = gemm_tn8(gy, Rows8(xv, xs), Rows8(av, as_), bits=bits, g_out=gz)
+            gw = gemm_tn8(gy, rows8_of(xv, xs), rows8_of(av, as_), bits=bits, g_out=gz)
         else:
             gz = _open_entries(gy, bits)
         if need[0] or need[1]:
@@ -338,10 +338,7 @@ def _checkpoint(name, checkpoint, allowed_rows, *xs):
     return rows
 
 
-@torch.compiler.disable
-def project(x: torch.Tensor, w: torch.Tensor, checkpoint=None) -> torch.Tensor:
-    """x @ w^T.  ``checkpoint="int8"``: x waits for the backward in 8 bits (or ``checkpoint=quantize_rows(x)``, when those
-    rows are at hand), from which the weight gradient is taken; differentiable once."""
+def _project(x, w, checkpoint):
     _require("project", x, w)
     if x.dtype == torch.bfloat16:
         x, w = x.contiguous(), w.contiguous()
@@ -353,10 +350,7 @@ def project(x: torch.Tensor, w: torch.Tensor, checkpoint=None) -> torch.Tensor:
     return _ProjectKept.apply(x, w, rows)
 
 
-@torch.compiler.disable
-def update(x: torch.Tensor, aggr: torch.Tensor, w_out: torch.Tensor, checkpoint=None) -> torch.Tensor:
-    """relu(x @ w_out[:, :F]^T + aggr @ w_out[:, F:]^T).  ``checkpoint="int8"``: x and aggr wait for the backward in 8
-    bits and the relu in one bit per entry; differentiable once."""
+def _update(x, aggr, w_out, checkpoint):
     _require("update", x, aggr, w_out)
     if x.dtype == torch.bfloat16:
         x, aggr = x.contiguous(), aggr.contiguous()
@@ -367,6 +361,21 @@ def update(x: torch.Tensor, aggr: torch.Tensor, w_out: torch.Tensor, checkpoint=
         raise ValueError(f"dense.update: w_out must have shape [M, {x.size(1) + aggr.size(1)}] and aggr {x.size(0)} rows, "
                          f"got {tuple(w_out.shape)} and {tuple(aggr.shape)}")
     return _UpdateKept.apply(x, aggr, w_out)
+
+
+_marked_project, _marked_update = torch.compiler.disable(_project), torch.compiler.disable(_update)
+
+
+def project(x: torch.Tensor, w: torch.Tensor, checkpoint=None) -> torch.Tensor:
+    """x @ w^T.  ``checkpoint="int8"``: x waits for the backward in 8 bits (or ``checkpoint=quantize_rows(x)``, when those
+    rows are at hand), from which the weight gradient is taken; differentiable once."""
+    return (_marked_project if torch.compiler.is_compiling() else _project)(x, w, checkpoint)
+
+
+def update(x: torch.Tensor, aggr: torch.Tensor, w_out: torch.Tensor, checkpoint=None) -> torch.Tensor:
+    """relu(x @ w_out[:, :F]^T + aggr @ w_out[:, F:]^T).  ``checkpoint="int8"``: x and aggr wait for the backward in 8
+    bits and the relu in one bit per entry; differentiable once."""
+    return (_marked_update if torch.compiler.is_compiling() else _update)(x, aggr, w_out, checkpoint)
 
 
 _ONES = {}

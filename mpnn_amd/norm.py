@@ -44,13 +44,15 @@ def _desc(plan, block, residual, gate, post_w, post_b, w, b, stream=None, normed
     d = _lib.BlockNormDesc()
     by_rows = plan.gate_kind > 1
     _DESC.pack_into(
-        d, 0, block.data_ptr(), _lib.leading(block), _p(residual), _lib.leading(residual), _p(gate), _lib.leading(gate) if by_rows else 0,
+        d, 0, block.data_ptr(), _lib.leading(block), _p(residual), _lib.leading(residual),
+        _p(gate), _lib.leading(gate) if by_rows else 0,
         _p(post_w), _p(post_b), _p(w), _p(b),
         block.size(0), block.size(1), _lib.dtype_code(block.dtype), plan.norm, plan.gate_kind, plan.post,
         plan.eps, plan.rs, plan.bs,
         _p(stream), _lib.leading(stream), _p(normed), _lib.leading(normed),
         _p(g_stream), _lib.leading(g_stream), _p(g_normed), _lib.leading(g_normed),
-        _p(g_block), _lib.leading(g_block), _p(g_residual), _lib.leading(g_residual), _p(g_gate), _lib.leading(g_gate) if by_rows else 0,
+        _p(g_block), _lib.leading(g_block), _p(g_residual), _lib.leading(g_residual),
+        _p(g_gate), _lib.leading(g_gate) if by_rows else 0,
         _p(g_post_w), _p(g_post_b), _p(g_w), _p(g_b), _p(partial))
     return d
 
@@ -127,7 +129,6 @@ def _gate_kind(gate, n: int, h: int):
     raise ValueError(f"gate must have shape [{h}], [1, {h}], [{n}, 1] or [{n}, {h}], got {tuple(gate.shape)}")
 
 
-@torch.compiler.disable
 def block_norm(block: torch.Tensor, residual: torch.Tensor | None = None, *, norm: str = "rms", eps: float = 1e-5,
                post_norm: bool = False, post_weight: torch.Tensor | None = None, post_bias: torch.Tensor | None = None,
                gate: torch.Tensor | None = None, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -138,6 +139,13 @@ def block_norm(block: torch.Tensor, residual: torch.Tensor | None = None, *, nor
     ``norm``: "rms" or "layer"; weights and biases [H] are optional.  ``gate`` multiplies the branch: [H] (one value per
     channel), [N, 1] (per node) or [N, H].  ``residual=None`` counts as zeros.  float32 or bfloat16 (all operands
     alike), 1 <= H <= 2048, any number of rows, rows at any stride; differentiable once with respect to every tensor."""
+    call = _marked if torch.compiler.is_compiling() else _block_norm
+    return call(block, residual, norm, eps, post_norm, post_weight, post_bias, gate, weight, bias, residual_scale,
+                branch_scale, outputs)
+
+
+def _block_norm(block, residual, norm, eps, post_norm, post_weight, post_bias, gate, weight, bias, residual_scale, branch_scale,
+                outputs):
     _lib.require_device(block, "block")
     _lib.dtype_code(block.dtype)
     if block.dim() != 2 or not 1 <= block.size(1) <= MAX_WIDTH:
@@ -164,8 +172,12 @@ def block_norm(block: torch.Tensor, residual: torch.Tensor | None = None, *, nor
         _operand("gate", gate, block, gate.shape)
         plan.gate_kind, gate = _gate_kind(gate, n, h)
     c = lambda t: None if t is None else t.contiguous()
-    tensors = (_lib.rows_in_place(block), None if residual is None else _lib.rows_in_place(residual), gate, c(post_weight), c(post_bias), c(weight), c(bias))
+    r = _lib.rows_in_place
+    tensors = (r(block), None if residual is None else r(residual), gate, c(post_weight), c(post_bias), c(weight), c(bias))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return _BlockNorm.apply(plan, *tensors)
     stream, normed = _forward(plan, *tensors)
     return (stream, normed) if outputs == "both" else (stream if normed is None else normed)
+
+
+_marked = torch.compiler.disable(_block_norm)      # for a tracing compiler: one graph break, no tracing into the operator

@@ -72,11 +72,16 @@ def _padded(v: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _new(n: int, k: int, device) -> Rows8:
+def rows8_of(values: torch.Tensor, scale: torch.Tensor) -> Rows8:
+    """Rows8 of parts that this module laid out itself (nothing is checked or copied)."""
     r = Rows8.__new__(Rows8)
-    r.values = torch.empty((n, _pitch(k)), dtype=torch.int8, device=device)[:, :k]
-    r.scale = torch.empty(n, dtype=torch.float32, device=device)
+    r.values, r.scale = values, scale
     return r
+
+
+def _new(n: int, k: int, device) -> Rows8:
+    return rows8_of(torch.empty((n, _pitch(k)), dtype=torch.int8, device=device)[:, :k],
+                    torch.empty(n, dtype=torch.float32, device=device))
 
 
 def _check_rows(name: str, x: torch.Tensor) -> None:
@@ -86,11 +91,21 @@ def _check_rows(name: str, x: torch.Tensor) -> None:
         raise ValueError(f"{name} must have shape [N, K] with 1 <= K <= {MAX_WIDTH}, got {tuple(x.shape)}")
 
 
-@torch.compiler.disable
 def quantize_rows(x: torch.Tensor) -> Rows8:
     """The rows of ``x`` (float32 or bfloat16 [N, K], any row stride) in 8 bits.  No gradient passes through."""
+    return (_marked_quantize if torch.compiler.is_compiling() else _checked_quantize)(x)
+
+
+def _checked_quantize(x: torch.Tensor) -> Rows8:
     _check_rows("x", x)
-    x = _lib.rows_in_place(x.detach())
+    return to_rows8(_lib.rows_in_place(x.detach()))
+
+
+_marked_quantize = torch.compiler.disable(_checked_quantize)
+
+
+def to_rows8(x: torch.Tensor) -> Rows8:
+    """quantize_rows of a checked matrix whose rows lie in place."""
     n, k = x.shape
     r = _new(n, k, x.device)
     _lib.check(_lib.load().mpnn_quantize_rows(_lib.ptr(x), _lib.leading(x), _lib.dtype_code(x.dtype), n, k,
@@ -99,13 +114,16 @@ def quantize_rows(x: torch.Tensor) -> Rows8:
     return r
 
 
-@torch.compiler.disable
 def linear_int8(x, weight: Rows8, bias: torch.Tensor | None = None, relu: bool = False,
                 dtype: torch.dtype | None = None) -> torch.Tensor:
     """``act(x @ weight^T + bias)`` on 8-bit rows with exact integer sums: x [N, K] as ``Rows8``, or in float32 / bfloat16
     (taken to 8 bits on the way, one scale per row); ``weight`` [M, K] one scale per output channel, made once with
     ``quantize_rows(w)``.  The result is ``dtype`` (x's own by default, float32 for ``Rows8``); ``bias`` [M] of that dtype.
     For answering only: no gradient."""
+    return (_marked_linear if torch.compiler.is_compiling() else _linear_int8)(x, weight, bias, relu, dtype)
+
+
+def _linear_int8(x, weight, bias, relu, dtype):
     held = isinstance(x, Rows8)
     if not isinstance(weight, Rows8):
         raise TypeError(f"weight must be Rows8 (quantize_rows(w)), got {type(weight).__name__}")
@@ -141,6 +159,9 @@ def linear_int8(x, weight: Rows8, bias: torch.Tensor | None = None, relu: bool =
                                     _lib.ptr(bias), _lib.ptr(y), m, code, n, k, m, 1 if relu else 0, _lib.ptr(space),
                                     _lib.stream_handle(x.device)), "mpnn_linear_int8")
     return y
+
+
+_marked_linear = torch.compiler.disable(_linear_int8)
 
 
 def kept_linear(x: torch.Tensor, w: torch.Tensor, x2: torch.Tensor | None = None, relu: bool = False):
