@@ -39,35 +39,29 @@ class _Plan:
     __slots__ = ("norm", "post", "gate_kind", "eps", "rs", "bs", "outputs")
 
 
-def _desc(plan, block, residual, gate, post_w, post_b, w, b, stream=None, normed=None, g_stream=None, g_normed=None,
-          g_block=None, g_residual=None, g_gate=None, g_post_w=None, g_post_b=None, g_w=None, g_b=None, partial=None):
-    d = _lib.BlockNormDesc()
-    by_rows = plan.gate_kind > 1
-    _DESC.pack_into(
-        d, 0, block.data_ptr(), _lib.leading(block), _p(residual), _lib.leading(residual),
-        _p(gate), _lib.leading(gate) if by_rows else 0,
-        _p(post_w), _p(post_b), _p(w), _p(b),
-        block.size(0), block.size(1), _lib.dtype_code(block.dtype), plan.norm, plan.gate_kind, plan.post,
-        plan.eps, plan.rs, plan.bs,
-        _p(stream), _lib.leading(stream), _p(normed), _lib.leading(normed),
-        _p(g_stream), _lib.leading(g_stream), _p(g_normed), _lib.leading(g_normed),
-        _p(g_block), _lib.leading(g_block), _p(g_residual), _lib.leading(g_residual),
-        _p(g_gate), _lib.leading(g_gate) if by_rows else 0,
-        _p(g_post_w), _p(g_post_b), _p(g_w), _p(g_b), _p(partial))
-    return d
-
-
 def _forward(plan, block, residual, gate, post_w, post_b, w, b):
-    lib = _lib.load()
     n, h = block.shape
     stream = normed = None
     if plan.outputs != "normed":
         stream = torch.empty((n, h), dtype=block.dtype, device=block.device)
     if plan.outputs != "stream":
         normed = torch.empty((n, h), dtype=block.dtype, device=block.device)
-    d = _desc(plan, block, residual, gate, post_w, post_b, w, b, stream=stream, normed=normed)
-    _lib.check(lib.mpnn_block_norm_fwd(d, _lib.stream_handle(block.device)), "mpnn_block_norm_fwd")
+    d = _lib.BlockNormDesc()
+    _DESC.pack_into(d, 0, *_inputs(plan, n, h, block, residual, gate, post_w, post_b, w, b),
+                    _p(stream), h, _p(normed), h, *_NO_GRADIENTS)
+    _lib.check(_lib.load().mpnn_block_norm_fwd(d, _lib.stream_handle(block.device)), "mpnn_block_norm_fwd")
     return stream, normed
+
+
+_NO_GRADIENTS = (0,) * 15
+
+
+def _inputs(plan, n, h, block, residual, gate, post_w, post_b, w, b):
+    """The fields both directions share (through branch_scale)."""
+    ld = _lib.leading
+    return (block.data_ptr(), ld(block), _p(residual), ld(residual), _p(gate), ld(gate) if plan.gate_kind > 1 else 0,
+            _p(post_w), _p(post_b), _p(w), _p(b), n, h, _lib.dtype_code(block.dtype), plan.norm, plan.gate_kind, plan.post,
+            plan.eps, plan.rs, plan.bs)
 
 
 class _BlockNorm(torch.autograd.Function):
@@ -95,25 +89,28 @@ class _BlockNorm(torch.autograd.Function):
         g_normed = None if g_normed is None else _lib.rows_in_place(g_normed)
         lib = _lib.load()
         n, h = block.shape
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and ctx.needs_input_grad[1 + i] else None
-                for i, t in enumerate(tensors)]
-        sums = plan.gate_kind == 1 and outs[2] is not None or any(o is not None for o in outs[3:])
+        outs = [torch.empty_like(t, memory_format=torch.contiguous_format)
+                if t is not None and need else None for t, need in zip(tensors, ctx.needs_input_grad[1:])]
+        g_block, g_residual, g_gate, g_post_w, g_post_b, g_w, g_b = outs
         partial = None
-        if sums:
-            floats = lib.mpnn_block_norm_partial_floats(n, h, _lib.dtype_code(block.dtype))
-            partial = torch.empty(floats, dtype=torch.float32, device=block.device)
-        d = _desc(plan, *tensors, g_stream=g_stream, g_normed=g_normed, g_block=outs[0], g_residual=outs[1],
-                  g_gate=outs[2], g_post_w=outs[3], g_post_b=outs[4], g_w=outs[5], g_b=outs[6], partial=partial)
+        if (plan.gate_kind == 1 and g_gate is not None) or not (g_post_w is g_post_b is g_w is g_b is None):
+            partial = torch.empty(lib.mpnn_block_norm_partial_floats(n, h, _lib.dtype_code(block.dtype)),
+                                  dtype=torch.float32, device=block.device)
+        ld = _lib.leading
+        d = _lib.BlockNormDesc()
+        _DESC.pack_into(d, 0, *_inputs(plan, n, h, *tensors), 0, 0, 0, 0, _p(g_stream), ld(g_stream), _p(g_normed), ld(g_normed),
+                        _p(g_block), h, _p(g_residual), h, _p(g_gate), 1 if plan.gate_kind == 2 else h,
+                        _p(g_post_w), _p(g_post_b), _p(g_w), _p(g_b), _p(partial))
         _lib.check(lib.mpnn_block_norm_bwd(d, _lib.stream_handle(block.device)), "mpnn_block_norm_bwd")
         return (None, *outs)
 
 
-def _operand(name, t, like, shape):
+def _refuse(name, t, like, shape):
+    """Why ``t`` cannot stand next to ``like``."""
     _lib.require_device(t, name)
     if t.dtype != like.dtype or t.device != like.device:
         raise TypeError(f"{name} must be {like.dtype} on {like.device} like block, got {t.dtype} on {t.device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _gate_kind(gate, n: int, h: int):
@@ -159,17 +156,15 @@ def _block_norm(block, residual, norm, eps, post_norm, post_weight, post_bias, g
     if outputs == "stream" and (weight is not None or bias is not None):
         raise ValueError('weight and bias belong to the normed output, which outputs="stream" leaves out')
     n, h = block.shape
-    if residual is not None:
-        _operand("residual", residual, block, block.shape)
-    vector = torch.Size((h,))
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)):
-        if t is not None:
-            _operand(name, t, block, vector)
+    dtype, device = block.dtype, block.device
+    for name, t, shape in (("residual", residual, (n, h)), ("post_weight", post_weight, (h,)), ("post_bias", post_bias, (h,)),
+                           ("weight", weight, (h,)), ("bias", bias, (h,)), ("gate", gate, None)):
+        if t is not None and (t.dtype != dtype or t.device != device or (shape is not None and t.shape != shape)):
+            _refuse(name, t, block, shape)
     plan = _Plan()
     plan.norm, plan.post, plan.eps, plan.outputs = NORMS[norm], int(bool(post_norm)), float(eps), outputs
     plan.rs, plan.bs, plan.gate_kind = float(residual_scale), float(branch_scale), 0
     if gate is not None:
-        _operand("gate", gate, block, gate.shape)
         plan.gate_kind, gate = _gate_kind(gate, n, h)
     c = lambda t: None if t is None else t.contiguous()
     r = _lib.rows_in_place

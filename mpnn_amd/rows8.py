@@ -164,13 +164,19 @@ def _linear_int8(x, weight, bias, relu, dtype):
 _marked_linear = torch.compiler.disable(_linear_int8)
 
 
+_FITS = {}     # shapes of kept_linear -> whether its kernel takes them
+
+
 def kept_linear(x: torch.Tensor, w: torch.Tensor, x2: torch.Tensor | None = None, relu: bool = False):
     """bfloat16 act(x @ w[:, :K]^T [+ x2 @ w[:, K:]^T]) with the inputs' 8-bit rows and the relu's bits from the same pass:
     (y, rows of x, rows of x2 or None, bits or None).  None where the shapes or layouts do not fit the kernel."""
     lib = _lib.load()
     n, k = x.shape
     m, k2 = w.size(0), (x2.size(1) if x2 is not None else 0)
-    if not lib.mpnn_kept_linear_fits(k, k2, m):
+    fits = _FITS.get((k, k2, m))
+    if fits is None:
+        fits = _FITS[(k, k2, m)] = bool(lib.mpnn_kept_linear_fits(k, k2, m))
+    if not fits:
         return None
     for t in (x, w, x2):
         if t is not None and (t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16):
