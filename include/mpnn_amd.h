@@ -642,7 +642,8 @@ int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
  * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * (x_scale[n] * w_scale[m]) + bias[m]); the sum is exact.  x_dtype
  *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits first, in the
  *   workspace (mpnn_linear_int8_workspace_bytes, 16-byte aligned).  W [M, ldw] 8-bit rows with w_scale [M]; bias [M]
- *   of y_dtype or NULL.  8-bit rows 16-byte aligned, strides multiples of 16; K <= 8192.
+ *   of y_dtype or NULL.  8-bit rows 16-byte aligned, strides multiples of 16 and (mpnn_linear_int8) at most
+ *   2^22; K <= 8192, M <= 2^20.
  * mpnn_gemm_tn8         dW[M, K + K2] = sum_n (G * open)[n, :]^T [scale[n] Q[n, :] | scale2[n] Q2[n, :]]
  *   G, dW, Gout of dtype; bits (mpnn_relu_bits of the layer's output) or NULL select the entries of G that count; Gout
  *   (optional, [N, M]) receives G * open.  Q2, scale2: optional (K2 = 0).  8-bit rows 4-byte aligned; row strides at

@@ -8,14 +8,13 @@
 // by every kernel here.  Weights are the first matrix operand, rows of x the second, so that a lane's results are
 // consecutive outputs of one row.  Bytes behind column K count as zeros on x's side, whatever the weights hold there.
 //
-// Three kernels:
+// Two kernels:
 //   rows    K <= 512, weights resident in LDS: x is read once as it lies, taken to 8 bits in registers and multiplied
 //           from there.  Bound by memory: 4 M rows of 128 -> 256 in 0.64 ms (bfloat16, 4.8 TB/s) and 1.19 ms (float32, 5.2
 //           TB/s; a copy reaches 4.9), Flickr's 89,250 of 500 -> 192 in 56 us (float32, 4.4 TB/s).
 //   tiles   both sides staged through LDS in steps of 128 bytes by asynchronous copies.  65,536 x 1024 -> 2048 to
 //           bfloat16 in 216 us (1270 TOP/s), 4096^3 in 80 us (1710 TOP/s).  What bounds it: operand reads from LDS (192
 //           KiB per step of 128 and CU, three quarters of the matrix cores' time) and, for short K, the results.
-//   thin    few rows: a wave per 32 x 32 outputs, operands from memory as they lie.  Bound by latency.
 #include "common.h"
 #include "rows8.h"
 
@@ -25,6 +24,7 @@ namespace {
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kI8MaxK = 8192;
+constexpr int kI8MaxM = 1 << 20;
 
 constexpr int kI8MaxTileLd = 1 << 22;   // bytes from row to row: a tile's rows are reached by 32-bit offsets
 
@@ -252,46 +252,6 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
   }
 }
 
-// ------------------------------------------------------------------------------------------------------------- thin
-// A block owns 32 rows x 128 outputs, a wave 32 x 32 of them.
-template <typename Y>
-__global__ void __launch_bounds__(kBlock) k_linear_i8_thin(I8Args a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int i32 = lane & 31, half = lane >> 5;
-  const int64_t n0 = (int64_t)blockIdx.x * 32;
-  const int m0 = (int)blockIdx.y * 128 + 32 * wave;
-  if (m0 >= a.M) return;
-  const int64_t row = n0 + i32 < a.N ? n0 + i32 : a.N - 1;
-  const int Kp = (a.K + 15) & ~15;
-  const int8_t* xp = static_cast<const int8_t*>(a.x) + row * a.ldx;
-  const int8_t* wp = a.w + (int64_t)(m0 + i32 < a.M ? m0 + i32 : a.M - 1) * a.ldw;
-  i32x16 acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0;
-#pragma unroll 8
-  for (int k0 = 0; k0 < Kp; k0 += 32) {
-    const int k = k0 + 16 * half;
-    const int off = k < Kp ? k : 0;
-    const i32x4 x = keep_bytes(*reinterpret_cast<const i32x4*>(xp + off), a.K - k);
-    acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const i32x4*>(wp + off), x, acc, 0, 0, 0);
-  }
-  if (n0 + i32 >= a.N) return;
-  const float xs = a.xs[row];
-  Y* y = static_cast<Y*>(a.y) + row * a.ldy;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int m = m0 + 8 * q + 4 * half;
-    if (m >= a.M) continue;
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int mj = m + j < a.M ? m + j : a.M - 1;
-      v[j] = finish(acc[4 * q + j], xs * a.ws[mj], a.bias ? scalar_to_f32(static_cast<const Y*>(a.bias)[mj]) : 0.f, a.relu);
-    }
-    store_outputs<Y, 4>(y + m, v, a.M - m, a.wide_out);
-  }
-}
-
 // ------------------------------------------------------------------------------------------------------------ tiles
 // A block of WN x WM waves owns WN * 32 TN rows x WM * 64 outputs; a wave TN x 2 tiles of 32 x 32.  Steps of PC 16-byte
 // pieces of K (8 or 4): rows lie in LDS PC pieces apart, their pieces in an order that depends on the row, so that the 8
@@ -454,21 +414,24 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
 }
 
 // --------------------------------------------------------------------------------------------------------- dispatch
-enum class I8Kernel { kRows, kThin, kTiles };
+// LDS bytes of 32 output columns in the rows kernel: weights, scales, biases.
+constexpr int rows_per32(int ks) { return 32 * (ks * 64 + 16 + 8); }
 
-// Rows: the row in registers (K <= 512) and the weights in at most two slices of a CU's LDS (x is read once per slice),
-// or so few rows that reading them again does not count.  Thin: fewer rows than fill the smaller tile twice.
-I8Kernel i8_kernel(int64_t N, int K, int M) {
-  if (K <= 512) {
-    const int pitch = (K <= 64 ? 1 : K <= 128 ? 2 : K <= 256 ? 4 : 8) * 64 + 16 + 8;
-    if (N <= 1024 || (int64_t)((M + 31) / 32 * 32) * pitch <= 2 * kI8RowsLds) return I8Kernel::kRows;
-  }
-  return N <= 256 ? I8Kernel::kThin : I8Kernel::kTiles;
+// Rows or tiles (whose x is taken to 8 bits by a pass of its own first).  The rows kernel reads x once per slice of weights
+// that fits the LDS.  Up to 256 columns it wins with one or two slices, or with few rows: 64 -> 2048 (two slices) takes 4 us
+// for 18 rows and 231 for 262,144, tiles 7.5 and 264; 256 -> 512 (two) 5.3 and 115 against 8.2 and 116.  Wider rows leave it
+// 8 waves per CU: it wins with one slice (1 M rows of 512 -> 128: 252 us, the quantising pass alone 300) and with very few
+// rows (512 -> 2048: 7.7 against 10.0 us for 18), and loses with more (65,536 rows of 512 -> 512, three slices: 69 against 49).
+bool i8_by_rows(int64_t N, int K, int M) {
+  if (K > 512) return false;
+  const int ks = K <= 64 ? 1 : K <= 128 ? 2 : K <= 256 ? 4 : 8;
+  const int64_t bytes = (int64_t)((M + 31) / 32) * rows_per32(ks);
+  return ks < 8 ? bytes <= 2 * kI8RowsLds || N <= 4096 : bytes <= kI8RowsLds || N <= 32;
 }
 
 template <typename X, typename Y, int KS, bool WIDE>
 int32_t launch_rows(const I8Args& a, hipStream_t stream) {
-  const int m32 = (a.M + 31) / 32, per32 = 32 * (KS * 64 + 16 + 8);
+  const int m32 = (a.M + 31) / 32, per32 = rows_per32(KS);
   const int64_t row_blocks = (a.N + 127) / 128;     // 8 waves of 16 rows
   // weights: as few slices as fit, more of them when the rows alone would leave CUs without work
   int slices = (m32 * per32 + kI8RowsLds - 1) / kI8RowsLds;
@@ -521,21 +484,16 @@ int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
 }
 
 template <typename Y>
-int32_t launch_i8(const I8Args& a, I8Kernel kernel, int x_dtype, bool wide_in, hipStream_t stream) {
-  if (kernel == I8Kernel::kRows) {
+int32_t launch_i8(const I8Args& a, bool rows, int x_dtype, bool wide_in, hipStream_t stream) {
+  if (rows) {
     if (x_dtype == MPNN_I8) return rows_of<int8_t, Y, true>(a, stream);
     if (x_dtype == MPNN_F32) return wide_in ? rows_of<float, Y, true>(a, stream) : rows_of<float, Y, false>(a, stream);
     return wide_in ? rows_of<bf16_t, Y, true>(a, stream) : rows_of<bf16_t, Y, false>(a, stream);
   }
-  if (kernel == I8Kernel::kThin) {
-    if ((a.M + 127) / 128 > 65535) return fail(MPNN_E_INVALID, "mpnn_linear_int8: M=%d", a.M);
-    const dim3 grid((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 127) / 128));
-    k_linear_i8_thin<Y><<<grid, kBlock, 0, stream>>>(a);
-    MPNN_LAUNCH_CHECK("k_linear_i8_thin");
-    return MPNN_OK;
-  }
-  // tiles of 256 x 256 if they fill the CUs, of 128 x 128 otherwise
-  if (((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, 2, 4, 4, 8>(a, stream);
+  // Tiles of 256 x 256 where they fill the CUs (16,384 rows of 500 -> 1024, 256 tiles: 30 us, with tiles of 128 x 128 32) and
+  // are not half empty; of 128 x 128 otherwise (16,384 of 512 -> 512, 128 large tiles: 18 us against 23; 65,536 of 2048 -> 64:
+  // 103 against 112).
+  if (a.M > 128 && ((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, 2, 4, 4, 8>(a, stream);
   return launch_tiles<Y, 2, 2, 2, 8>(a, stream);
 }
 
@@ -547,8 +505,8 @@ using namespace mpnn;
 extern "C" {
 
 int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_t x_dtype) {
-  if (N < 0 || K < 1 || K > kI8MaxK || M < 1) return -1;
-  if (x_dtype == MPNN_I8 || i8_kernel(N, K, M) == I8Kernel::kRows) return 0;
+  if (N < 0 || K < 1 || K > kI8MaxK || M < 1 || M > kI8MaxM) return -1;
+  if (x_dtype == MPNN_I8 || i8_by_rows(N, K, M)) return 0;
   return N * ((K + 15) / 16 * 16) + align_up(N * 4, 16);
 }
 
@@ -557,18 +515,16 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
                          int32_t K, int32_t M, int32_t relu, void* workspace, mpnn_stream_t stream) {
   if ((x_dtype != MPNN_F32 && x_dtype != MPNN_BF16 && x_dtype != MPNN_I8) || (y_dtype != MPNN_F32 && y_dtype != MPNN_BF16))
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: dtypes %d, %d", x_dtype, y_dtype);
-  if (N < 0 || K < 1 || K > kI8MaxK || M < 1 || M > (1 << 24))
-    return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld K=%d M=%d (K up to %d)", (long long)N, K, M, kI8MaxK);
+  if (N < 0 || K < 1 || K > kI8MaxK || M < 1 || M > kI8MaxM)
+    return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld K=%d M=%d (K up to %d, M up to %d)", (long long)N, K, M, kI8MaxK, kI8MaxM);
   const int Kp = (K + 15) / 16 * 16;
   if (ldx < (x_dtype == MPNN_I8 ? Kp : K) || ldw < Kp || ldy < M) return fail(MPNN_E_INVALID, "mpnn_linear_int8: leading dimension too small");
   if (N == 0) return MPNN_OK;
-  const I8Kernel kernel = i8_kernel(N, K, M);
-  const bool take = x_dtype != MPNN_I8 && kernel != I8Kernel::kRows;     // to 8 bits in a pass of its own
+  const bool rows = i8_by_rows(N, K, M), take = x_dtype != MPNN_I8 && !rows;     // to 8 bits in a pass of its own
   if (!X || !W || !w_scale || !Y || (x_dtype == MPNN_I8 && !x_scale) || (take && !workspace))
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: null pointer argument");
   if (((uintptr_t)W & 15) || (ldw & 15) || (x_dtype == MPNN_I8 && (((uintptr_t)X & 15) || (ldx & 15))) || ((uintptr_t)workspace & 15))
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: 8-bit rows and the workspace must be 16-byte aligned");
-  if ((N + 31) / 32 > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld", (long long)N);
   const int vec = y_dtype == MPNN_BF16 ? 8 : 4;
   const int wide_out = ((uintptr_t)Y & 15) == 0 && ldy % vec == 0;
   I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out};
@@ -581,8 +537,8 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
   }
   const int xvec = x_dtype == MPNN_BF16 ? 8 : 4;
   const bool wide_in = K % xvec == 0 && ldx % xvec == 0 && ((uintptr_t)X & 15) == 0;
-  return y_dtype == MPNN_BF16 ? launch_i8<bf16_t>(a, kernel, x_dtype, wide_in, stream)
-                              : launch_i8<float>(a, kernel, x_dtype, wide_in, stream);
+  return y_dtype == MPNN_BF16 ? launch_i8<bf16_t>(a, rows, x_dtype, wide_in, stream)
+                              : launch_i8<float>(a, rows, x_dtype, wide_in, stream);
 }
 
 }  // extern "C"

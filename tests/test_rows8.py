@@ -218,6 +218,27 @@ def test_linear_int8_strides_special_rows_and_no_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,k,m", [(18, 11, 128), (300, 700, 300), (16384, 520, 1024)])
+def test_linear_int8_captured_and_on_another_stream(n, k, m):
+    from mpnn_amd import linear_int8, quantize_rows
+    x, w8 = randn(n, k, seed=1).cuda(), quantize_rows(randn(m, k, seed=2).cuda())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = linear_int8(x, w8)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        x.mul_(-1.5)
+        want = linear_int8(x, w8)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = linear_int8(x, w8)
+        torch.cuda.current_stream().wait_stream(side)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want) and torch.equal(other, want)
+
+
+@pytest.mark.gpu
 def test_linear_int8_refusals():
     from mpnn_amd import Rows8, linear_int8, quantize_rows
     w8 = quantize_rows(randn(8, 16).cuda())
