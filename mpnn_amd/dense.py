@@ -21,7 +21,10 @@ _SCRATCH = {}
 
 def _scratch(n: int, device) -> torch.Tensor:
     """Partial-tile scratch of the weight-gradient products, one buffer per (device, stream): calls on one stream
-    reuse it in stream order, calls on different streams never share it."""
+    reuse it in stream order, calls on different streams never share it.  A call that is captured gets its own: graphs
+    recorded on one stream may be replayed side by side."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(n, dtype=torch.float32, device=device)
     key = (device, _lib.stream_handle(device))
     buf = _SCRATCH.get(key)
     if buf is None or buf.numel() < n:
@@ -35,7 +38,9 @@ _WSPLIT = {}
 
 def _wsplit(nbytes: int, device) -> torch.Tensor:
     """Room for the split weight images of one NT product.  One buffer per device and stream-ordered reuse: every
-    call rewrites it before its own GEMM reads it, on the stream both run on."""
+    call rewrites it before its own GEMM reads it, on the stream both run on.  (Captured calls: see _scratch.)"""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device, _lib.stream_handle(device))
     buf = _WSPLIT.get(key)
     if buf is None or buf.numel() < nbytes:

@@ -51,6 +51,7 @@ def _checkpoint(checkpoint):
 
 class MPNNLayerCat(torch.nn.Module):
     """``checkpoint="int8"`` (no counterpart in the reference): what the layer keeps for its backward waits in 8 bits."""
+    checkpoint = None        # (modules unpickled from before the option have no attribute of their own)
 
     def __init__(self, in_channels, edge_channels, out_channels, checkpoint=None):
         super().__init__()
@@ -73,6 +74,7 @@ class MPNNLayerCat(torch.nn.Module):
 
 class MPNNLayerSum(torch.nn.Module):
     """``checkpoint="int8"`` (no counterpart in the reference): what the layer keeps for its backward waits in 8 bits."""
+    checkpoint = None        # (modules unpickled from before the option have no attribute of their own)
 
     def __init__(self, in_channels, edge_channels, out_channels, checkpoint=None):
         super().__init__()

@@ -198,3 +198,53 @@ def test_option_is_checked_without_a_gpu():
         MPNNLayerCat(8, 4, 8, checkpoint=True)
     assert MPNN(20, 32, 7, checkpoint="int8").layers[1].checkpoint == "int8"
     assert MPNN(20, 32, 7).layers[0].checkpoint is None
+
+
+@pytest.mark.gpu
+def test_captured_products_replay_side_by_side():
+    """Two graphs recorded one after the other, replayed at once on two streams: neither uses the other's workspaces."""
+    from mpnn_amd.dense import project
+    n = 60000
+    xs = [torch.randn(n, 64, device="cuda").requires_grad_() for _ in range(2)]
+    ws = [torch.randn(200, 64, device="cuda").requires_grad_() for _ in range(2)]
+    gy = torch.randn(n, 200, device="cuda")
+
+    def step(k):
+        y = project(xs[k], ws[k], checkpoint="int8")
+        return (y.detach(), *torch.autograd.grad(y, (xs[k], ws[k]), gy))
+
+    want = [step(0), step(1)]
+    graphs, held = [], []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(step(k))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, h in zip(want, held):
+        assert all(torch.equal(a, b) for a, b in zip(w, h))
+
+
+@pytest.mark.gpu
+def test_operators_inside_a_traced_function():
+    """A tracing compiler breaks its graph at the operators and takes their eager results."""
+    from mpnn_amd import block_norm, linear_int8, quantize_rows
+    from mpnn_amd.dense import project, update
+    x, w = torch.randn(300, 64, device="cuda"), torch.randn(64, 64, device="cuda")
+    wo, w8 = torch.randn(64, 128, device="cuda"), quantize_rows(w)
+
+    def run(x):
+        y = update(x, project(x, w, checkpoint="int8"), wo, checkpoint="int8")
+        stream, u = block_norm(y * 2, x)
+        with torch.no_grad():
+            return stream + 1, linear_int8(u, w8)
+
+    traced = torch.compile(run, backend="eager")
+    for a, b in zip(traced(x), run(x)):
+        assert torch.equal(a, b)
