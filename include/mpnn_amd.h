@@ -41,7 +41,7 @@ enum {
   MPNN_E_CAPACITY = -4   /* an output array's stated capacity is too small */
 };
 
-#define MPNN_ABI_VERSION 20
+#define MPNN_ABI_VERSION 21
 
 /* Library self-description. */
 int32_t mpnn_abi_version(void);
@@ -658,15 +658,16 @@ int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_
 int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const float* x_scale, const void* W, int64_t ldw,
                          const float* w_scale, const void* bias, void* Y, int64_t ldy, int32_t y_dtype, int64_t N,
                          int32_t K, int32_t M, int32_t relu, void* workspace, mpnn_stream_t stream);
-/* bfloat16 Y = act(X W[:, :K]^T [+ X2 W[:, K:]^T]) that also leaves the inputs' rows in 8 bits (Q, scale [, Q2, scale2], as
+/* Y = act(X W[:, :K]^T [+ X2 W[:, K:]^T]) that also leaves the inputs' rows in 8 bits (Q, scale [, Q2, scale2], as
  * mpnn_quantize_rows does) and, with `bits`, the relu's bits (as mpnn_relu_bits of Y), in one pass over the inputs.
- * K, K2, M multiples of 8, K and K2 at most 256 and weights that fit the LDS (mpnn_kept_linear_fits tells); K2 = 0: one
- * input.  Everything 16-byte aligned, row strides too. */
-int32_t mpnn_kept_linear_fits(int32_t K, int32_t K2, int32_t M);
-int32_t mpnn_kept_linear_bf16(const void* X, int64_t ldx, int32_t K, void* Q, int64_t ldq, float* scale, const void* X2,
-                              int64_t ldx2, int32_t K2, void* Q2, int64_t ldq2, float* scale2, const void* W, int64_t ldw,
-                              void* Y, int64_t ldy, void* bits, int64_t N, int32_t M, int32_t relu,
-                              mpnn_stream_t stream);
+ * K and K2 at most 256 and weights that fit the LDS (mpnn_kept_linear_fits tells); K2 = 0: one input.  8-bit rows and
+ * inputs 16-byte aligned, row strides too.  float32: K and K2 multiples of 4, Y as mpnn_gemm_nt's to the bit.  bfloat16:
+ * K, K2, M multiples of 8, W and Y 16-byte aligned, their row strides too. */
+int32_t mpnn_kept_linear_fits(int32_t K, int32_t K2, int32_t M, int32_t dtype);
+int32_t mpnn_kept_linear(const void* X, int64_t ldx, int32_t K, void* Q, int64_t ldq, float* scale, const void* X2,
+                         int64_t ldx2, int32_t K2, void* Q2, int64_t ldq2, float* scale2, const void* W, int64_t ldw,
+                         void* Y, int64_t ldy, void* bits, int64_t N, int32_t M, int32_t relu, int32_t dtype,
+                         mpnn_stream_t stream);
 int64_t mpnn_gemm_tn8_scratch_floats(int64_t N, int32_t M, int32_t K, int32_t K2, int32_t dtype);
 int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bits, const void* Q, int64_t ldq,
                       const float* scale, int32_t K, const void* Q2, int64_t ldq2, const float* scale2, int32_t K2,

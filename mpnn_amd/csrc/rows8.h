@@ -53,31 +53,45 @@ __device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int lef
   }
 }
 
-// Results of a wave on their way to memory: ROWS rows x 64 outputs in LDS, from where whole row segments leave (128 bytes
+// 16 bytes to a row that is not read here again.  Rows of whole 64-byte lines leave past the L2, which keeps the operands;
+// other rows share lines with their neighbours, and the L2 must put the parts together: 1 M x 100 float32 results from
+// 8-bit rows of 100 take 207 us past it and 147 through it, 1 M x 128 100 and 129.
+__device__ __forceinline__ void store_chunk(void* p, i32x4 v, bool whole) {
+  if (whole) {
+    asm volatile("");   // on either side: keeps the two stores apart (joined, both would go through the L2)
+    __builtin_nontemporal_store(v, static_cast<i32x4*>(p));
+    asm volatile("");
+  } else {
+    *static_cast<i32x4*>(p) = v;
+  }
+}
+
+// Results of a wave on their way to memory: ROWS rows x COLS outputs in LDS, from where whole row segments leave (128 bytes
 // in bfloat16, 256 in float32; stores of 64 bytes per row took 1.65 instead of 1.20 ms for 4 M rows of 256 in float32).
 // 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread.  Only
 // the wave that owns the patch touches it.
-template <typename Y, int ROWS>
+template <typename Y, int ROWS, int COLS = 64>
 struct Patch {
-  static constexpr int VEC = 16 / sizeof(Y), CHUNKS = 64 / VEC, BYTES = ROWS * 64 * sizeof(Y);
+  static constexpr int VEC = 16 / sizeof(Y), CHUNKS = COLS / VEC, BYTES = ROWS * COLS * sizeof(Y);
   char* base;
   __device__ __forceinline__ void put(int row, int chunk, const float (&v)[VEC]) const {
-    store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (64 * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
+    store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (COLS * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
   }
-  // To rows r0 .. of y [N, ldy], outputs m .. m + 63 of which those below `end` exist; wide: 16-byte stores are possible.
+  // To rows r0 .. of y [N, ldy], outputs m .. m + COLS - 1 of which those below `end` exist; wide: 16-byte stores are possible.
   __device__ __forceinline__ void leave(void* y, int64_t ldy, int64_t N, int64_t r0, int m, int end, bool wide) const {
     const int lane = threadIdx.x & 63;
+    const bool whole = (ldy * sizeof(Y)) % 64 == 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int q = 0; q < ROWS * CHUNKS / 64; ++q) {
       const int r = q * (64 / CHUNKS) + lane / CHUNKS, chunk = lane % CHUNKS;
-      const i32x4 v = *reinterpret_cast<const i32x4*>(base + r * (64 * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
+      const i32x4 v = *reinterpret_cast<const i32x4*>(base + r * (COLS * (int)sizeof(Y)) + ((chunk ^ r) & (CHUNKS - 1)) * 16);
       const int left = end - m - chunk * VEC;
       if (r0 + r >= N || left <= 0) continue;
       Y* const p = static_cast<Y*>(y) + (r0 + r) * ldy + m + chunk * VEC;
       if (wide && left >= VEC) {
-        __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(p));   // not read here again: the L2 keeps the operands
+        store_chunk(p, v, whole);
       } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)

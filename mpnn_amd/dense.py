@@ -245,7 +245,7 @@ class _ProjectKept(torch.autograd.Function):
     def forward(ctx, x, w, rows):
         y = None
         if ctx.needs_input_grad[1] and rows is None:
-            both = kept_linear(x, w) if x.dtype == torch.bfloat16 else None      # one pass over x
+            both = kept_linear(x, w)                                             # one pass over x
             y, rows = (both[0], both[1]) if both is not None else (None, to_rows8(_lib.rows_in_place(x)))
         if ctx.needs_input_grad[1]:
             ctx.save_for_backward(w, rows.values, rows.scale)
@@ -274,7 +274,7 @@ class _UpdateKept(torch.autograd.Function):
         if bf and not bf16_ok(w_out):
             w_out = w_out.contiguous()
         want = ctx.needs_input_grad[2]
-        both = kept_linear(x, w_out, aggr, relu=True) if bf and want else None   # one pass over x and aggr
+        both = kept_linear(x, w_out, aggr, relu=True) if want else None          # one pass over x and aggr
         if both is not None:
             y, rx, ra, bits = both
         else:

@@ -203,7 +203,7 @@ class _KeptLayerFn(torch.autograd.Function):
         a, b = ab[:, :h], ab[:, h:]
         ea_s, ea_t = ops._prepare(a, b, edge_attr, w_edge, graph)
         aggr, cnt, maskbits = ops._run_forward(a, b, ea_s, w_edge, graph.by_dst, graph, True)
-        both = kept_linear(x, w_out, aggr, relu=True) if bf else None
+        both = kept_linear(x, w_out, aggr, relu=True)
         if both is not None:
             y, rx, ra, bits = both
         else:

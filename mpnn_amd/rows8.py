@@ -164,31 +164,29 @@ def _linear_int8(x, weight, bias, relu, dtype):
 _marked_linear = torch.compiler.disable(_linear_int8)
 
 
-_FITS = {}     # shapes of kept_linear -> whether its kernel takes them
-
-
 def kept_linear(x: torch.Tensor, w: torch.Tensor, x2: torch.Tensor | None = None, relu: bool = False):
-    """bfloat16 act(x @ w[:, :K]^T [+ x2 @ w[:, K:]^T]) with the inputs' 8-bit rows and the relu's bits from the same pass:
-    (y, rows of x, rows of x2 or None, bits or None).  None where the shapes or layouts do not fit the kernel."""
+    """act(x @ w[:, :K]^T [+ x2 @ w[:, K:]^T]) with the inputs' 8-bit rows and the relu's bits from the same pass:
+    (y, rows of x, rows of x2 or None, bits or None).  None where the shapes or layouts do not fit the kernel.  In float32
+    y is gemm_nt's to the bit."""
     lib = _lib.load()
+    code = _lib.dtype_code(x.dtype)
     n, k = x.shape
     m, k2 = w.size(0), (x2.size(1) if x2 is not None else 0)
-    fits = _FITS.get((k, k2, m))
-    if fits is None:
-        fits = _FITS[(k, k2, m)] = bool(lib.mpnn_kept_linear_fits(k, k2, m))
-    if not fits:
+    if not lib.mpnn_kept_linear_fits(k, k2, m, code):
         return None
+    unit = 8 if code == _lib.MPNN_BF16 else 4      # elements of 16 bytes
     for t in (x, w, x2):
-        if t is not None and (t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16):
+        if t is not None and (t.stride(1) != 1 or t.stride(0) % unit or t.data_ptr() % 16
+                              or (t.size(0) > 1 and t.stride(0) < t.size(1))):
             return None
     r, r2 = _new(n, k, x.device), (_new(n, k2, x.device) if x2 is not None else None)
-    y = torch.empty((n, m), dtype=torch.bfloat16, device=x.device)
+    y = torch.empty((n, m), dtype=x.dtype, device=x.device)
     bits = torch.empty((n, (m + 31) // 32), dtype=torch.int32, device=x.device) if relu else None
     q2, ld2, s2 = (_lib.ptr(r2.values), r2.pitch, _lib.ptr(r2.scale)) if r2 is not None else (None, 0, None)
-    _lib.check(lib.mpnn_kept_linear_bf16(_lib.ptr(x), _lib.leading(x), k, _lib.ptr(r.values), r.pitch, _lib.ptr(r.scale),
-                                         _lib.ptr(x2), _lib.leading(x2), k2, q2, ld2, s2, _lib.ptr(w), _lib.leading(w),
-                                         _lib.ptr(y), m, _lib.ptr(bits), n, m, 1 if relu else 0,
-                                         _lib.stream_handle(x.device)), "mpnn_kept_linear_bf16")
+    _lib.check(lib.mpnn_kept_linear(_lib.ptr(x), _lib.leading(x), k, _lib.ptr(r.values), r.pitch, _lib.ptr(r.scale),
+                                    _lib.ptr(x2), _lib.leading(x2), k2, q2, ld2, s2, _lib.ptr(w), _lib.leading(w),
+                                    _lib.ptr(y), m, _lib.ptr(bits), n, m, 1 if relu else 0, code,
+                                    _lib.stream_handle(x.device)), "mpnn_kept_linear")
     return y, r, r2, bits
 
 

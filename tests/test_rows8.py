@@ -558,3 +558,87 @@ def test_entry_points_refuse_before_any_launch():
                 dict(q=p + 2), dict(ldq=18), dict(dt=1, ldg=9), dict(dt=1, m=7), dict(dt=1, g=p + 2)):
         assert tn(**bad) == -1, bad
     assert lib.mpnn_gemm_tn8_scratch_floats(-1, 8, 8, 0, 0) == -1
+
+
+# the kernel holds every value as three bfloat16 pieces (exact: 8 + 8 + 8 bits) and leaves out the products second x third,
+# third x second and third x third: at most (2 * 2^-7 * 2^-15 + 2^-30) |x w|; six products per pair are added, each
+# addition off by at most 2^-23 of a partial sum (a rounding or a truncation)
+def kept_f32_bound(k, size):
+    return (6 * k * 1.02 * 2.0 ** -23 + 2.0 ** -21 + 2.0 ** -30) * size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,k2,m", [(1, 4, 0, 1), (1, 12, 0, 128), (31, 32, 0, 40), (32, 40, 8, 32), (33, 64, 64, 64), (63, 36, 0, 33),
+                                      (65, 24, 20, 96), (100, 128, 64, 64), (129, 60, 124, 64), (257, 128, 128, 64), (500, 252, 0, 37),
+                                      (1000, 128, 0, 256), (2049, 20, 100, 100), (3001, 72, 32, 104), (777, 100, 52, 70),
+                                      (40000, 64, 64, 64), (70000, 128, 0, 128)])
+@pytest.mark.parametrize("relu", [False, True])
+def test_kept_linear_in_float32(n, k, k2, m, relu):
+    from mpnn_amd.dense import gemm_nt
+    from mpnn_amd.rows8 import kept_linear, quantize_rows, relu_bits
+    x = randn(n, k, seed=n).cuda()
+    x2 = randn(n, k2, seed=n + 1).cuda() if k2 else None
+    w = randn(m, k + k2, seed=n + 2).cuda()
+    if n > 20:
+        x[3] = 0
+        x[5, 2] = float("inf")
+        x[n - 1, k - 1] = float("nan")
+    both = torch.cat([x] + ([x2] if k2 else []), dim=1).double()
+    fine = torch.isfinite(both).all(dim=1)
+    want = both[fine] @ w.double().t()
+    size = both[fine].abs() @ w.double().abs().t()
+    want = want.clamp_min(0) if relu else want
+    plain = gemm_nt(x, w[:, :k], x2, w[:, k:] if k2 else None, relu=relu)
+    wider = torch.zeros((n, k + 8), device="cuda")             # rows inside a wider matrix
+    wider[:, 4:k + 4] = x
+    for xs in (x, wider[:, 4:k + 4]):
+        y, r, r2, bits = kept_linear(xs, w, x2, relu=relu)
+        for rows, t in ((r, x), (r2, x2)):
+            if t is not None:
+                q = quantize_rows(t)
+                assert torch.equal(rows.values, q.values) and torch.equal(rows.scale.nan_to_num(nan=-1), q.scale.nan_to_num(nan=-1))
+                assert torch.equal(torch.as_strided(rows.values, (n, rows.pitch), (rows.pitch, 1)), torch.as_strided(q.values, (n, q.pitch), (q.pitch, 1)))
+        assert bool(((y[fine].double() - want).abs() <= kept_f32_bound(k + k2, size)).all())
+        assert torch.equal(y[fine], plain[fine])
+        assert torch.equal(bits, relu_bits(y)) if relu else bits is None
+        if n > 20:
+            assert not torch.isfinite(y[5]).all()
+            assert y[n - 1].isnan().all()
+    wider[:, 1:k + 1] = x
+    assert kept_linear(wider[:, 1:k + 1], w, x2) is None       # off a 16-byte boundary
+
+
+@pytest.mark.gpu
+def test_float32_inputs_that_take_the_separate_passes(monkeypatch):
+    from mpnn_amd.dense import project, update
+    from mpnn_amd.rows8 import kept_linear
+    x, a = randn(300, 128).cuda(), randn(300, 64, seed=1).cuda()
+    w = randn(64, 192, seed=2).cuda()
+    assert kept_linear(torch.cat([x, x, x], dim=1), torch.cat([w, w], dim=1)) is None       # 384 wide
+    assert kept_linear(x[:, :11].contiguous(), w[:, :11].contiguous()) is None
+    for mode in (None, "f32"):
+        if mode:
+            monkeypatch.setenv("MPNN_GEMM", mode)
+        assert (kept_linear(x, w, a) is None) == (mode == "f32")
+        assert torch.equal(update(x, a, w.requires_grad_(), checkpoint="int8"), update(x, a, w))
+        x11, w11 = x[:, :11].contiguous(), w.detach()[:, :11].contiguous().requires_grad_()
+        assert torch.equal(project(x11, w11, checkpoint="int8"), project(x11, w11))
+
+
+def test_kept_linear_refuses_before_any_launch():
+    """Addresses are never followed here: every call is rejected on the host."""
+    lib = _lib.load()
+    p = 1 << 20
+    base = dict(x=p, ldx=64, k=64, q=p, ldq=64, s=p, x2=p, ldx2=32, k2=32, q2=p, ldq2=32, s2=p, w=p, ldw=96, y=p, ldy=64, bits=None,
+                n=4, m=64, relu=0, dt=0, st=None)
+    call = lambda **k: lib.mpnn_kept_linear(*{**base, **k}.values())
+    shared = (dict(n=-1), dict(k=0), dict(k2=-1), dict(m=0), dict(dt=2), dict(k=264, ldx=264, ldq=272, ldw=296), dict(m=4104, ldy=4104),
+              dict(ldx=60), dict(ldx2=24), dict(ldw=88), dict(ldy=56), dict(ldq=48), dict(ldq2=16), dict(q=p + 8), dict(ldq=72), dict(ldq2=40),
+              dict(x=None), dict(q=None), dict(s=None), dict(x2=None), dict(q2=None), dict(s2=None), dict(w=None), dict(y=None),
+              dict(x=p + 4), dict(x2=p + 8))
+    for bad in shared + (dict(k=62), dict(k2=30), dict(ldx=66), dict(ldx2=34), dict(m=1024, ldy=1024)):
+        assert call(**bad) == -1, bad
+    for bad in shared + (dict(k=60), dict(m=60), dict(ldx=68), dict(ldw=100), dict(ldy=68), dict(w=p + 2), dict(y=p + 8)):
+        assert call(**{**bad, "dt": bad.get("dt", 1)}) == -1, bad
+    assert call(n=0) == 0 and call(n=0, dt=1) == 0
+    assert lib.mpnn_kept_linear_fits(128, 0, 256, 0) == 1 and lib.mpnn_kept_linear_fits(128, 128, 128, 0) == 0
