@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import Rows8, gemm_tn8, kept_linear, relu_bits, rows8_of, to_rows8
+from .rows8 import Rows8, gemm_tn8, kept_linear, relu_bits, rows8_again, to_rows8
 
 _SCRATCH = {}
 
@@ -259,7 +259,7 @@ class _ProjectKept(torch.autograd.Function):
         w, values, scale = ctx.saved_tensors
         g = _upstream(g)
         gx = _kit(g.dtype)[0](g, w.t().contiguous()) if ctx.needs_input_grad[0] else None
-        gw = gemm_tn8(g, rows8_of(values, scale)) if ctx.needs_input_grad[1] else None
+        gw = gemm_tn8(g, rows8_again(values, scale)) if ctx.needs_input_grad[1] else None
         return gx, gw, None
 
 
@@ -294,7 +294,7 @@ class _UpdateKept(torch.autograd.Function):
         gz = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device) if need[0] or need[1] else None
         gx = ga = gw = None
         if need[2]:
-            gw = gemm_tn8(gy, rows8_of(xv, xs), rows8_of(av, as_), bits=bits, g_out=gz)
+            gw = gemm_tn8(gy, rows8_again(xv, xs), rows8_again(av, as_), bits=bits, g_out=gz)
         else:
             gz = _open_entries(gy, bits)
         if need[0] or need[1]:

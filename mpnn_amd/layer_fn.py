@@ -31,7 +31,7 @@ from . import islands, ops
 from .dense import gemm_nt, gemm_nt_bf16, gemm_tn, gemm_tn_bf16
 from .graph import MPGraph
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import gemm_tn8, kept_linear, relu_bits, rows8_of, to_rows8
+from .rows8 import gemm_tn8, kept_linear, relu_bits, rows8_again, to_rows8
 
 
 def fused_x(dtype, f: int, h: int) -> bool:
@@ -224,12 +224,12 @@ class _KeptLayerFn(torch.autograd.Function):
         bf = gy.dtype == torch.bfloat16
         nt = gemm_nt_bf16 if bf else gemm_nt
         f, h = xv.size(1), w_out.size(0)
-        rx, n = rows8_of(xv, xs), xv.size(0)
+        rx, n = rows8_again(xv, xs), xv.size(0)
         gy = gy.contiguous()
         if gy.data_ptr() % 16:
             gy = gy.clone()
         gz = torch.empty_like(gy)
-        g_wout = gemm_tn8(gy, rx, rows8_of(av, as_), bits=bits, g_out=gz)
+        g_wout = gemm_tn8(gy, rx, rows8_again(av, as_), bits=bits, g_out=gz)
         wt_out = w_out.t().contiguous()                   # [F+H, H]
         g_ab = torch.empty((n, 2 * h), dtype=gy.dtype, device=gy.device)
         cnt = (cnt8, cnt_big)

@@ -79,6 +79,11 @@ def rows8_of(values: torch.Tensor, scale: torch.Tensor) -> Rows8:
     return r
 
 
+def rows8_again(values: torch.Tensor, scale: torch.Tensor) -> Rows8:
+    """Rows8 of what an autograd node saved: a hook on saved tensors may have brought it back in another layout."""
+    return rows8_of(values if _in_place(values) else _padded(values), scale.contiguous())
+
+
 def _new(n: int, k: int, device) -> Rows8:
     return rows8_of(torch.empty((n, _pitch(k)), dtype=torch.int8, device=device)[:, :k],
                     torch.empty(n, dtype=torch.float32, device=device))

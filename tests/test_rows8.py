@@ -642,3 +642,21 @@ def test_kept_linear_refuses_before_any_launch():
         assert call(**{**bad, "dt": bad.get("dt", 1)}) == -1, bad
     assert call(n=0) == 0 and call(n=0, dt=1) == 0
     assert lib.mpnn_kept_linear_fits(128, 0, 256, 0) == 1 and lib.mpnn_kept_linear_fits(128, 128, 128, 0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40, 500])
+def test_saved_rows_that_come_back_in_another_layout(n):
+    """A hook that moves what waits for the backward to the host returns it without the padding behind its rows."""
+    from mpnn_amd.dense import project, update
+    x, a = randn(n, 100).cuda().requires_grad_(), randn(n, 37, seed=1).cuda().requires_grad_()
+    w, wo = randn(64, 100, seed=2).cuda().requires_grad_(), randn(50, 137, seed=3).cuda().requires_grad_()
+
+    def grads():
+        y, z = project(x, w, checkpoint="int8"), update(x, a, wo, checkpoint="int8")
+        return lambda: torch.autograd.grad([y, z], [x, a, w, wo], [torch.ones_like(y), torch.ones_like(z)])
+    want = grads()()
+    with torch.autograd.graph.save_on_cpu():
+        later = grads()
+    for p, q in zip(later(), want):
+        assert torch.equal(p, q)
