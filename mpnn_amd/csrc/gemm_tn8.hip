@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kBlock) k_tn8_sums(const float* __restrict__ p
 template <typename T>
 __global__ void __launch_bounds__(kBlock) k_gemm_tn8_few(Tn8Args a, T* __restrict__ dW, int64_t ldw) {
   const int ktot = a.K + a.K2;
-  const int c = (int)blockIdx.x * 64 + (threadIdx.x & 63), m = (int)blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int c = (int)blockIdx.y * 64 + (threadIdx.x & 63), m = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= a.M) return;
   const bool second = c >= a.K;
   const int8_t* q = second ? a.q2 : a.q;
@@ -433,7 +433,7 @@ int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bit
   if (N < 0 || M < 1 || K < 1 || K2 < 0 || M > kTn8MaxLd || K > kTn8MaxLd || K2 > kTn8MaxLd)
     return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: N=%lld M=%d K=%d K2=%d", (long long)N, M, K, K2);
   const int64_t ktot = (int64_t)K + K2;
-  if (M * ktot > (1 << 30)) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: M=%d x %lld outputs", M, (long long)ktot);
+  if (M * ktot > (1 << 30) || (ktot + 63) / 64 > 65535) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: M=%d x %lld outputs", M, (long long)ktot);
   if (!dW || lddw < ktot) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: dW is null or lddw below K + K2");
   const Tn8Plan p = tn8_plan(N, M, K, K2, bf16);
   if (N > 0) {
@@ -458,8 +458,7 @@ int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bit
     a.ktiles = p.ktiles;
     a.slabs = (int)((N + p.slab_rows - 1) / p.slab_rows);
     if (N < kTn8Rows) {
-      if ((M + 3) / 4 > 65535) return fail(MPNN_E_INVALID, "mpnn_gemm_tn8: M=%d", M);
-      const dim3 grid((unsigned)((ktot + 63) / 64), (unsigned)((M + 3) / 4));
+      const dim3 grid((unsigned)((M + 3) / 4), (unsigned)((ktot + 63) / 64));
       if (bf16) k_gemm_tn8_few<bf16_t><<<grid, kBlock, 0, stream>>>(a, static_cast<bf16_t*>(dW), lddw);
       else k_gemm_tn8_few<float><<<grid, kBlock, 0, stream>>>(a, static_cast<float*>(dW), lddw);
       MPNN_LAUNCH_CHECK("k_gemm_tn8_few");

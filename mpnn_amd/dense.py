@@ -343,6 +343,12 @@ def _checkpoint(name, checkpoint, allowed_rows, *xs):
     return rows
 
 
+def _gradient_fits(name, w):
+    """The weight gradient from 8-bit rows has its limits: told here, not in the backward."""
+    if w.size(0) > 1 << 21 or w.numel() > 1 << 30:
+        raise ValueError(f"dense.{name}: weights of at most {1 << 21} rows and {1 << 30} entries with kept rows, got {tuple(w.shape)}")
+
+
 def _project(x, w, checkpoint):
     _require("project", x, w)
     if x.dtype == torch.bfloat16:
@@ -352,6 +358,9 @@ def _project(x, w, checkpoint):
     rows = _checkpoint("project", checkpoint, True, x)
     if w.dim() != 2 or w.size(1) != x.size(1):
         raise ValueError(f"dense.project: w must have shape [M, {x.size(1)}], got {tuple(w.shape)}")
+    _gradient_fits("project", w)
+    if not torch.is_grad_enabled():      # nothing waits for a backward
+        return _Project.apply(x, w)
     return _ProjectKept.apply(x, w, rows)
 
 
@@ -365,6 +374,9 @@ def _update(x, aggr, w_out, checkpoint):
     if x.size(0) != aggr.size(0) or w_out.dim() != 2 or w_out.size(1) != x.size(1) + aggr.size(1):
         raise ValueError(f"dense.update: w_out must have shape [M, {x.size(1) + aggr.size(1)}] and aggr {x.size(0)} rows, "
                          f"got {tuple(w_out.shape)} and {tuple(aggr.shape)}")
+    _gradient_fits("update", w_out)
+    if not torch.is_grad_enabled():
+        return _Update.apply(x, aggr, w_out)
     return _UpdateKept.apply(x, aggr, w_out)
 
 

@@ -660,3 +660,31 @@ def test_saved_rows_that_come_back_in_another_layout(n):
         later = grads()
     for p, q in zip(later(), want):
         assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_weights_with_many_rows_and_few_rows_of_x():
+    from mpnn_amd.dense import project
+    m = 262148                                            # more blocks than one grid dimension of 65,535 takes
+    x, w = randn(3, 4).cuda(), randn(m, 4, seed=1).cuda().requires_grad_()
+    g = randn(3, m, seed=2).cuda()
+    (gw,) = torch.autograd.grad(project(x, w, checkpoint="int8"), [w], g)
+    from mpnn_amd.rows8 import quantize_rows
+    want = g.double().t() @ quantize_rows(x).dequantize(torch.float32).double()
+    size = g.double().abs().t() @ x.double().abs()
+    # three products of once rounded factors (scale, g * scale; q is exact) and their sums
+    assert bool(((gw.double() - want).abs() <= 6 * 2.0 ** -24 * size + 1e-30).all())
+
+
+@pytest.mark.gpu
+def test_kept_rows_only_where_something_waits():
+    from mpnn_amd.dense import project, update
+    x, a = randn(300, 64).cuda(), randn(300, 32, seed=1).cuda()
+    w, wo = randn(64, 64, seed=2).cuda().requires_grad_(), randn(32, 96, seed=3).cuda().requires_grad_()
+    with torch.no_grad():
+        y, z = project(x, w, checkpoint="int8"), update(x, a, wo, checkpoint="int8")
+    assert not y.requires_grad and not z.requires_grad
+    assert torch.equal(y, project(x, w, checkpoint="int8")) and torch.equal(z, update(x, a, wo, checkpoint="int8"))
+    big = torch.empty(1, device="cuda").expand((1 << 21) + 1, 64)
+    with pytest.raises(ValueError, match="at most"):
+        project(x, big, checkpoint="int8")
