@@ -246,7 +246,7 @@ class _ProjectKept(torch.autograd.Function):
         y = None
         if ctx.needs_input_grad[1] and rows is None:
             both = kept_linear(x, w)                                             # one pass over x
-            y, rows = (both[0], both[1]) if both is not None else (None, to_rows8(_lib.rows_in_place(x)))
+            y, rows = (both[0], both[1]) if both is not None else (None, to_rows8(x))
         if ctx.needs_input_grad[1]:
             ctx.save_for_backward(w, rows.values, rows.scale)
         else:
@@ -279,7 +279,7 @@ class _UpdateKept(torch.autograd.Function):
             y, rx, ra, bits = both
         else:
             y = _kit(x.dtype)[0](x, w_out[:, :f], aggr, w_out[:, f:], relu=True)
-            rx, ra = (to_rows8(_lib.rows_in_place(x)), to_rows8(_lib.rows_in_place(aggr))) if want else (None, None)
+            rx, ra = (to_rows8(x), to_rows8(aggr)) if want else (None, None)
             bits = relu_bits(y)
         kept = (rx.values, rx.scale, ra.values, ra.scale) if want else (None,) * 4
         ctx.save_for_backward(w_out, bits, *kept)
@@ -359,6 +359,7 @@ def _project(x, w, checkpoint):
     if w.dim() != 2 or w.size(1) != x.size(1):
         raise ValueError(f"dense.project: w must have shape [M, {x.size(1)}], got {tuple(w.shape)}")
     _gradient_fits("project", w)
+    x = _lib.rows_in_place(x)
     if not torch.is_grad_enabled():      # nothing waits for a backward
         return _Project.apply(x, w)
     return _ProjectKept.apply(x, w, rows)
@@ -375,6 +376,7 @@ def _update(x, aggr, w_out, checkpoint):
         raise ValueError(f"dense.update: w_out must have shape [M, {x.size(1) + aggr.size(1)}] and aggr {x.size(0)} rows, "
                          f"got {tuple(w_out.shape)} and {tuple(aggr.shape)}")
     _gradient_fits("update", w_out)
+    x, aggr = _lib.rows_in_place(x), _lib.rows_in_place(aggr)
     if not torch.is_grad_enabled():
         return _Update.apply(x, aggr, w_out)
     return _UpdateKept.apply(x, aggr, w_out)

@@ -688,3 +688,17 @@ def test_kept_rows_only_where_something_waits():
     big = torch.empty(1, device="cuda").expand((1 << 21) + 1, 64)
     with pytest.raises(ValueError, match="at most"):
         project(x, big, checkpoint="int8")
+
+
+@pytest.mark.gpu
+def test_kept_calls_with_expanded_inputs():
+    from mpnn_amd.dense import project, update
+    row, a = randn(1, 64).cuda().requires_grad_(), randn(200, 32, seed=1).cuda()
+    w, wo = randn(48, 64, seed=2).cuda().requires_grad_(), randn(32, 96, seed=3).cuda().requires_grad_()
+    x = row.expand(200, 64)
+    for f, full in ((lambda t: project(t, w, checkpoint="int8"), w), (lambda t: update(t, a, wo, checkpoint="int8"), wo)):
+        y, y_full = f(x), f(x.contiguous())
+        assert torch.equal(y, y_full)
+        g = torch.ones_like(y)
+        for p, q in zip(torch.autograd.grad(y, [row, full], g), torch.autograd.grad(y_full, [row, full], g)):
+            assert torch.equal(p, q)
