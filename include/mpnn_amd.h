@@ -41,7 +41,7 @@ enum {
   MPNN_E_CAPACITY = -4   /* an output array's stated capacity is too small */
 };
 
-#define MPNN_ABI_VERSION 21
+#define MPNN_ABI_VERSION 22
 
 /* Library self-description. */
 int32_t mpnn_abi_version(void);
@@ -668,6 +668,11 @@ int32_t mpnn_kept_linear(const void* X, int64_t ldx, int32_t K, void* Q, int64_t
                          int64_t ldx2, int32_t K2, void* Q2, int64_t ldq2, float* scale2, const void* W, int64_t ldw,
                          void* Y, int64_t ldy, void* bits, int64_t N, int32_t M, int32_t relu, int32_t dtype,
                          mpnn_stream_t stream);
+/* Y = X W for W [K, M] as it lies (the input gradient of a Linear call: X the upstream gradient, W the weight), for widths that
+ * mpnn_kept_linear_fits(K, 0, M, dtype) takes.  X 16-byte aligned, its row stride too; in bfloat16 Y also.  float32: as
+ * mpnn_gemm_nt of W's transpose to the bit. */
+int32_t mpnn_gemm_nn(const void* X, int64_t ldx, const void* W, int64_t ldw, void* Y, int64_t ldy, int64_t N, int32_t K,
+                     int32_t M, int32_t dtype, mpnn_stream_t stream);
 int64_t mpnn_gemm_tn8_scratch_floats(int64_t N, int32_t M, int32_t K, int32_t K2, int32_t dtype);
 int32_t mpnn_gemm_tn8(const void* G, int64_t ldg, int32_t dtype, const void* bits, const void* Q, int64_t ldq,
                       const float* scale, int32_t K, const void* Q2, int64_t ldq2, const float* scale2, int32_t K2,

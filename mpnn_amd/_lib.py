@@ -15,7 +15,7 @@ MPNN_F32 = 0
 MPNN_BF16 = 1
 MPNN_U8 = 2
 MPNN_I8 = 3
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 LIB_PATH = os.environ.get("MPNN_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmpnn_amd.so")
 
@@ -166,8 +166,10 @@ SIGNATURES = {
                                    c_int64, c_int32, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "mpnn_kept_linear_fits": (c_int32, [c_int32, c_int32, c_int32, c_int32]),
     "mpnn_kept_linear": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32,
-                                        c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                                        c_int64, c_int32, c_int32, c_int32, c_void_p]),
+                                    c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                    c_int32, c_int32, c_int32, c_void_p]),
+    "mpnn_gemm_nn": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,
+                               c_void_p]),
     "mpnn_gemm_tn8_scratch_floats": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32]),
     "mpnn_gemm_tn8": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_void_p,
                                 c_int64, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,

@@ -16,6 +16,10 @@
 //              not fit go in two slices, and x is read once per slice.  Bound by the matrix cores: 4 M rows, 128 -> 256, in 1.70 ms
 //              (0.92 PFLOP/s of piece products, where a large bfloat16 product reaches 1.28; the separate passes 2.29), 128 -> 128
 //              in 0.94 (1.44); 1 M rows, 64 + 64 -> 64, in 197 us (330).
+//
+// Without kept rows the same kernels are the input gradient of those calls, y = x W for W as it lies [K, M]: brought into
+// place on its way to LDS, it saves the pass that transposes it (with that pass and gemm_nt: 18,432 x 64 -> 64 float32 16 us,
+// here 9; 4 M x 128 -> 256 bfloat16 0.66 and 0.59 ms, float32 1.83 and 1.63).
 #include "common.h"
 #include "rows8.h"
 
@@ -45,6 +49,7 @@ struct KeptArgs {
   uint8_t* bits;                    // optional
   int64_t N;
   int M, relu, wide_out;
+  int across;                       // the weights lie as [K, M]: y = x W (one input, nothing kept: the input gradient)
 };
 
 constexpr int kept_pitch(int ks) { return ks * 64 + 16; }   // bytes of a weight row in LDS: 16 more spread eight rows over the banks
@@ -166,12 +171,25 @@ __global__ void __launch_bounds__(kKeptThreads, kept_waves(KS1, KS2)) k_kept_lin
   // weights to LDS: output m of a pair of 16-row tiles t in row 16 t + r with m = 8 (r / 4) + 4 t + r % 4, so that a lane ends
   // with 8 consecutive outputs; zeros behind the widths (the other operand's zeros would not do: 0 * NaN)
   for (int idx = threadIdx.x; idx < m_pad * (KS * 4); idx += kKeptThreads) {
-    const int pos = idx / (KS * 4), c = idx - pos * (KS * 4), r = pos & 15;
+    int pos = idx / (KS * 4), c = idx - pos * (KS * 4);
+    if (KS2 == 0 && a.across) {     // neighbours in a row of W
+      c = idx / m_pad;
+      pos = idx - c * m_pad;
+    }
+    const int r = pos & 15;
     const int m = (pos & ~31) + 8 * (r >> 2) + 4 * ((pos >> 4) & 1) + (r & 3);
     const bool second = c >= KS1 * 4;
     const int k = (second ? c - KS1 * 4 : c) * 8;
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (m < a.M && k < (second ? a.b.K : a.a.K))
+    if (KS2 == 0 && a.across) {
+      if (m < a.M && k < a.a.K) {   // widths are multiples of 8
+        const bf16_t* w = static_cast<const bf16_t*>(a.w) + (int64_t)k * a.ldw + m;
+        uint32_t t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = w[e * a.ldw];
+        v = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+      }
+    } else if (m < a.M && k < (second ? a.b.K : a.a.K))
       v = *reinterpret_cast<const uint4*>(static_cast<const bf16_t*>(a.w) + (int64_t)m * a.ldw + (second ? a.a.K : 0) + k);
     *reinterpret_cast<uint4*>(lds + pos * PITCH + c * 16) = v;
   }
@@ -214,7 +232,7 @@ __global__ void __launch_bounds__(kKeptThreads, kept_waves(KS1, KS2)) k_kept_lin
       }
       if ((b & 32) || b + 32 >= m_pad) patch.leave(a.y, a.ldy, a.N, r0, b & ~63, a.M, true);
     }
-    keep_rows<KS1>(raw1, a.a, a.N, r0, patch_base);
+    if (a.a.q) keep_rows<KS1>(raw1, a.a, a.N, r0, patch_base);
     if constexpr (KS2 > 0) keep_rows<KS2>(raw2, a.b, a.N, r0, patch_base);
   }
 }
@@ -354,14 +372,21 @@ __global__ void __launch_bounds__(kKeptThreads, 2) k_kept_linear_f32(KeptArgs a,
   // weights to LDS, cut into pieces: output m of 32 in row 8 (m % 16 / 4) + 4 (m / 16) + m % 4, so that a lane ends with 16
   // consecutive outputs; zeros behind the widths
   for (int idx = threadIdx.x; idx < m_pad * (KS * 4); idx += kKeptThreads) {
-    const int pos = idx / (KS * 4), c = idx - pos * (KS * 4), k = c >> 1, ch = c & 1;
+    int pos = idx / (KS * 4), c = idx - pos * (KS * 4);
+    const bool across = KS2 == 0 && a.across;
+    if (across) {                   // neighbours in a row of W
+      c = idx / m_pad;
+      pos = idx - c * m_pad;
+    }
+    const int k = c >> 1, ch = c & 1;
     const int m = m_begin + (pos & ~31) + 16 * ((pos >> 2) & 1) + 4 * ((pos >> 3) & 3) + (pos & 3);
     const bool second = k >= 2 * KS1;
     const int col = (second ? k - 2 * KS1 : k) * 16 + 8 * ch, K = second ? a.b.K : a.a.K;
-    const float* w = static_cast<const float*>(a.w) + (int64_t)(m < a.M ? m : 0) * a.ldw + (second ? a.a.K : 0);
+    const int64_t along = across ? a.ldw : 1;      // from one contraction index to the next
+    const float* w = static_cast<const float*>(a.w) + (m < a.M ? m : 0) * (across ? 1 : a.ldw) + (second ? a.a.K : 0);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = m < a.M && col + e < K ? w[col + e] : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = m < a.M && col + e < K ? w[(col + e) * along] : 0.f;
     bf16x8 p[3];
     cut(v, p);
 #pragma unroll
@@ -374,7 +399,7 @@ __global__ void __launch_bounds__(kKeptThreads, 2) k_kept_linear_f32(KeptArgs a,
     bf16x8 x[2 * KS][3];
     if constexpr (!AHEAD) fetch_rows<KS1>(next1, a.a, row_of(tile), half());
     clear_tail<KS1>(next1, a.a, h);
-    if (blockIdx.y == 0) keep_rows<KS1>(next1, a.a, a.N, r0, patch_base);
+    if (blockIdx.y == 0 && a.a.q) keep_rows<KS1>(next1, a.a, a.N, r0, patch_base);
 #pragma unroll
     for (int k = 0; k < 2 * KS1; ++k) cut(next1.v[k], x[k]);
     if constexpr (KS2 > 0) {
@@ -465,6 +490,25 @@ int32_t launch_kept1_f32(const KeptArgs& a, hipStream_t stream) {
   return fail(MPNN_E_INVALID, "mpnn_kept_linear: no kernel for K=%d K2=%d", a.a.K, a.b.K);
 }
 
+int32_t launch_kept_any(KeptArgs& a, int32_t dtype, hipStream_t stream) {
+  const int steps = kept_steps(a.a.K);
+  if (dtype == MPNN_F32) {
+    a.wide_out = ((uintptr_t)a.y & 15) == 0 && a.ldy % 4 == 0;
+    switch (steps) {
+      case 1: return launch_kept1_f32<1>(a, stream);
+      case 2: return launch_kept1_f32<2>(a, stream);
+      case 4: return launch_kept1_f32<4>(a, stream);
+      default: return launch_kept1_f32<8>(a, stream);
+    }
+  }
+  switch (steps) {
+    case 1: return launch_kept1<1>(a, stream);
+    case 2: return launch_kept1<2>(a, stream);
+    case 4: return launch_kept1<4>(a, stream);
+    default: return launch_kept1<8>(a, stream);
+  }
+}
+
 }  // namespace
 }  // namespace mpnn
 
@@ -509,21 +553,26 @@ int32_t mpnn_kept_linear(const void* X, int64_t ldx, int32_t K, void* Q, int64_t
   a.y = Y; a.ldy = ldy;
   a.bits = static_cast<uint8_t*>(bits);
   a.N = N; a.M = M; a.relu = relu;
-  if (!bf16) {
-    a.wide_out = ((uintptr_t)Y & 15) == 0 && ldy % 4 == 0;
-    switch (kept_steps(K)) {
-      case 1: return launch_kept1_f32<1>(a, stream);
-      case 2: return launch_kept1_f32<2>(a, stream);
-      case 4: return launch_kept1_f32<4>(a, stream);
-      default: return launch_kept1_f32<8>(a, stream);
-    }
-  }
-  switch (kept_steps(K)) {
-    case 1: return launch_kept1<1>(a, stream);
-    case 2: return launch_kept1<2>(a, stream);
-    case 4: return launch_kept1<4>(a, stream);
-    default: return launch_kept1<8>(a, stream);
-  }
+  return launch_kept_any(a, dtype, stream);
+}
+
+int32_t mpnn_gemm_nn(const void* X, int64_t ldx, const void* W, int64_t ldw, void* Y, int64_t ldy, int64_t N, int32_t K,
+                     int32_t M, int32_t dtype, mpnn_stream_t stream) {
+  if (N < 0 || !mpnn_kept_linear_fits(K, 0, M, dtype))
+    return fail(MPNN_E_INVALID, "mpnn_gemm_nn: N=%lld K=%d M=%d dtype %d (see mpnn_kept_linear_fits)", (long long)N, K, M, dtype);
+  if (ldx < K || ldw < M || ldy < M) return fail(MPNN_E_INVALID, "mpnn_gemm_nn: leading dimension too small");
+  if (N == 0) return MPNN_OK;
+  if (!X || !W || !Y) return fail(MPNN_E_INVALID, "mpnn_gemm_nn: null pointer argument");
+  const int vec = dtype == MPNN_BF16 ? 8 : 4;
+  if (((uintptr_t)X & 15) || ldx % vec || (dtype == MPNN_BF16 && (((uintptr_t)Y & 15) || ldy % vec)))
+    return fail(MPNN_E_INVALID, "mpnn_gemm_nn: rows must be 16-byte aligned with strides that keep them so");
+  KeptArgs a;
+  memset(&a, 0, sizeof a);
+  a.a = KeptSeg{X, ldx, nullptr, 0, nullptr, K};
+  a.w = W; a.ldw = ldw;
+  a.y = Y; a.ldy = ldy;
+  a.N = N; a.M = M; a.across = 1;
+  return launch_kept_any(a, dtype, stream);
 }
 
 }  // extern "C"

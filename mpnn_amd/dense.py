@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import Rows8, gemm_tn8, kept_linear, relu_bits, rows8_again, to_rows8
+from .rows8 import Rows8, gemm_nn, gemm_tn8, kept_linear, relu_bits, rows8_again, to_rows8
 
 _SCRATCH = {}
 
@@ -258,7 +258,7 @@ class _ProjectKept(torch.autograd.Function):
     def backward(ctx, g):
         w, values, scale = ctx.saved_tensors
         g = _upstream(g)
-        gx = _kit(g.dtype)[0](g, w.t().contiguous()) if ctx.needs_input_grad[0] else None
+        gx = _across(g, w) if ctx.needs_input_grad[0] else None
         gw = gemm_tn8(g, rows8_again(values, scale)) if ctx.needs_input_grad[1] else None
         return gx, gw, None
 
@@ -298,16 +298,20 @@ class _UpdateKept(torch.autograd.Function):
         else:
             gz = _open_entries(gy, bits)
         if need[0] or need[1]:
-            nt = _kit(gy.dtype)[0]
-            wt = w_out.t().contiguous()
             if need[0] and need[1]:
-                g_both = nt(gz, wt)              # one pass over gz: the two gradients are column halves of it
+                g_both = _across(gz, w_out)      # one pass over gz: the two gradients are column halves of it
                 gx, ga = g_both[:, :f], g_both[:, f:]
             elif need[0]:
-                gx = nt(gz, wt[:f])
+                gx = _across(gz, w_out[:, :f])
             else:
-                ga = nt(gz, wt[f:])
+                ga = _across(gz, w_out[:, f:])
         return gx, ga, gw
+
+
+def _across(g, w):
+    """g @ w: from the weight as it lies where that fits, else by its transpose."""
+    y = gemm_nn(g, w)
+    return _kit(g.dtype)[0](g, w.t().contiguous()) if y is None else y
 
 
 def _open_entries(g, bits):

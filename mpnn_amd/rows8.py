@@ -195,6 +195,27 @@ def kept_linear(x: torch.Tensor, w: torch.Tensor, x2: torch.Tensor | None = None
     return y, r, r2, bits
 
 
+def gemm_nn(g: torch.Tensor, w: torch.Tensor):
+    """g @ w for w [K, M] as it lies, None where the widths or layouts do not fit the kernel.  In float32 it is
+    gemm_nt(g, w^T) to the bit."""
+    lib = _lib.load()
+    code = _lib.dtype_code(g.dtype)
+    (n, k), m = g.shape, w.size(1)
+    # float32 wider than 128: the pieces fill the registers (1 M x 256 -> 64: 295 us, by the transpose 287; 1 M x 128 -> 128: 238 and 278)
+    if code == _lib.MPNN_F32 and k > 128:
+        return None
+    if not lib.mpnn_kept_linear_fits(k, 0, m, code):
+        return None
+    ldg, ldw = _lib.leading(g), _lib.leading(w)
+    if (g.stride(1) != 1 or w.stride(1) != 1 or ldg % (8 if code == _lib.MPNN_BF16 else 4) or g.data_ptr() % 16
+            or (n > 1 and g.stride(0) < k) or (k > 1 and w.stride(0) < m)):
+        return None
+    y = torch.empty((n, m), dtype=g.dtype, device=g.device)
+    _lib.check(lib.mpnn_gemm_nn(_lib.ptr(g), ldg, _lib.ptr(w), ldw, _lib.ptr(y), m, n, k, m, code,
+                                _lib.stream_handle(g.device)), "mpnn_gemm_nn")
+    return y
+
+
 def relu_bits(y: torch.Tensor) -> torch.Tensor:
     """One bit per entry of a relu's output [N, M]: int32 [N, ceil(M / 32)], set where the relu is open."""
     n, m = y.shape

@@ -702,3 +702,49 @@ def test_kept_calls_with_expanded_inputs():
         g = torch.ones_like(y)
         for p, q in zip(torch.autograd.grad(y, [row, full], g), torch.autograd.grad(y_full, [row, full], g)):
             assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,m", [(1, 4, 1), (31, 32, 40), (33, 64, 11), (100, 128, 11), (129, 128, 64), (500, 124, 33), (1000, 100, 100),
+                                   (4099, 64, 128), (40000, 128, 128), (9000, 96, 256)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_input_gradient_from_the_weight_as_it_lies(n, k, m, dtype):
+    from mpnn_amd.dense import gemm_nt
+    from mpnn_amd.rows8 import gemm_nn
+    bf = dtype == torch.bfloat16
+    if bf:
+        k, m = (k + 7) // 8 * 8, (m + 7) // 8 * 8
+    g, w = randn(n, k, seed=n, dtype=dtype).cuda(), randn(k, m, seed=n + 1, dtype=dtype).cuda()
+    wider = torch.zeros((k, m + 5), dtype=dtype, device="cuda")       # a column slice of a wider weight, at any alignment
+    wider[:, 3:m + 3] = w
+    gw = torch.zeros((n, k + 8), dtype=dtype, device="cuda")
+    gw[:, :k] = g
+    if n > 20:
+        g[7, 1] = float("inf")
+        gw[7, 1] = float("inf")
+    fine = torch.isfinite(g).all(dim=1)
+    want, size = g[fine].double() @ w.double(), g[fine].double().abs() @ w.double().abs()
+    for gs, ws in ((g, w), (gw[:, :k], wider[:, 3:m + 3])):
+        y = gemm_nn(gs, ws)
+        if bf:
+            bound = 2 * k * U * size
+            assert bool(((y[fine].double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all())
+        else:
+            assert bool(((y[fine].double() - want).abs() <= kept_f32_bound(k, size)).all())
+            assert torch.equal(y[fine], gemm_nt(g, w.t().contiguous())[fine])
+        assert n <= 20 or not torch.isfinite(y[7]).any()
+    assert gemm_nn(g[:, 1:], w[1:]) is None                           # off a 16-byte boundary, and a width that does not fit
+    assert bf or gemm_nn(torch.ones((n, 256), device="cuda"), torch.ones((256, m), device="cuda")) is None
+
+
+def test_gemm_nn_refuses_before_any_launch():
+    """Addresses are never followed here: every call is rejected on the host."""
+    lib = _lib.load()
+    p = 1 << 20
+    base = dict(x=p, ldx=64, w=p, ldw=40, y=p, ldy=40, n=4, k=64, m=40, dt=0, st=None)
+    call = lambda **k: lib.mpnn_gemm_nn(*{**base, **k}.values())
+    for bad in (dict(n=-1), dict(k=0), dict(m=0), dict(k=62), dict(k=264, ldx=264), dict(dt=2), dict(ldx=60), dict(ldw=39), dict(ldy=39),
+                dict(x=None), dict(w=None), dict(y=None), dict(x=p + 4), dict(ldx=66), dict(dt=1, y=p + 8), dict(dt=1, ldy=44),
+                dict(dt=1, ldx=68), dict(dt=1, m=36), dict(k=128, ldx=128, m=4096, ldw=4096, ldy=4096)):
+        assert call(**bad) == -1, bad
+    assert call(n=0) == 0 and call(n=0, dt=1) == 0
