@@ -375,11 +375,12 @@ Tn8Plan tn8_plan(int64_t N, int M, int K, int K2, bool bf16) {
   p.wk = (p.ktiles > 1 && p.wm < 8) ? 2 : 1;
   p.wn = 8 / (p.wm * p.wk);
   p.slab_rows = kTn8Rows;
-  // one block per CU over all output tiles, at least two slabs each
+  // one block per CU over all output tiles, as many as there are slabs (two slabs each at least: 18,432 rows, 64 x [64 | 64]
+  // float32 18.5 us instead of 16.3, no faster with more rows)
   const int tiles = ((p.strips + p.wm - 1) / p.wm) * ((p.ktiles + p.wk - 1) / p.wk);
   int64_t blocks = 256 / tiles;
   const int64_t slabs = (N + p.slab_rows - 1) / p.slab_rows;
-  if (blocks > (slabs + 1) / 2) blocks = (slabs + 1) / 2;
+  if (blocks > slabs) blocks = slabs;
   if (blocks < 1) blocks = 1;
   p.blocks = (int)blocks;
   return p;
