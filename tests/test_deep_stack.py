@@ -248,3 +248,39 @@ def test_operators_inside_a_traced_function():
     traced = torch.compile(run, backend="eager")
     for a, b in zip(traced(x), run(x)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_matrices_beyond_32_bit_offsets(dtype):
+    """More than 2^31 entries: the last rows are what they are by themselves."""
+    from mpnn_amd import block_norm, linear_int8, quantize_rows
+    from mpnn_amd.dense import project
+    n, h, tail = (1 << 31) // 128 + 1001, 128, 1000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty((n, h), dtype=dtype, device="cuda").normal_(generator=gen)
+    w = torch.randn(64, h, device="cuda", generator=gen).to(dtype).requires_grad_()
+    last = x[-tail:].clone()
+
+    def ends(t):
+        return t[-tail:].clone()
+    stream, normed = block_norm(x, x, norm="layer", post_norm=True)
+    for p, q in zip((stream, normed), block_norm(last, last, norm="layer", post_norm=True)):
+        assert torch.equal(ends(p), q)
+    del stream, normed
+    rows, rows_last = quantize_rows(x), quantize_rows(last)
+    assert torch.equal(ends(rows.values), rows_last.values) and torch.equal(ends(rows.scale), rows_last.scale)
+    w8 = quantize_rows(torch.randn(h, h, device="cuda", generator=gen).to(dtype))
+    assert torch.equal(ends(linear_int8(x, w8)), linear_int8(last, w8))
+    assert torch.equal(ends(linear_int8(rows, w8)), linear_int8(rows_last, w8))
+    x.requires_grad_()
+    last.requires_grad_()
+    y, y_last = project(x, w, checkpoint="int8"), project(last, w, checkpoint="int8")
+    assert torch.equal(ends(y.detach()), y_last)
+    gy = torch.zeros((n, 64), dtype=dtype, device="cuda")
+    gy[-tail:] = torch.randn(tail, 64, device="cuda", generator=gen)
+    (gx, gw), (gx_last, gw_last) = (torch.autograd.grad(o, (i, w), g) for o, i, g in ((y, x, gy), (y_last, last, gy[-tail:])))
+    assert torch.equal(ends(gx), gx_last) and not gx[:-tail].any()
+    # the rows meet in other blocks: float32 sums of 1000 products each way, one rounding to the type
+    size = gy[-tail:].double().abs().t() @ rows_last.dequantize().double().abs()
+    assert bool(((gw - gw_last).double().abs() <= 2 * tail * 2.0 ** -24 * size + torch.finfo(dtype).eps * gw_last.double().abs()).all())
