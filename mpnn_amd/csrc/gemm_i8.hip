@@ -37,7 +37,7 @@ struct I8Args {
   void* y; int64_t ldy;
   int64_t N;
   int K, M, relu;
-  int wide_out;                    // 8 consecutive outputs can leave as 16-byte vectors
+  int width;                       // of the stores (store_width)
 };
 
 __device__ __forceinline__ float finish(int32_t acc, float scale, float bias, int relu) {
@@ -70,13 +70,15 @@ template <> struct XRaw<float> { float v[16]; };
 template <> struct XRaw<bf16_t> { uint32_t v[8]; };
 template <> struct XRaw<int8_t> { i32x4 v; };
 
-template <typename X, bool WIDE>
+// V elements of a row per load: the widest that the width, the address and the stride allow (89,250 bfloat16 rows of 500 -> 192:
+// 39 us in vectors of 4, 86 one by one).
+template <typename X, int V>
 __device__ __forceinline__ void load_x(const X* p, int s, int g, int K, XRaw<X>& r) {
   if constexpr (sizeof(X) == 4) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int k = 64 * s + 16 * q + 4 * g;
-      if constexpr (WIDE) {   // K is a multiple of 4
+      if constexpr (V == 4) {   // K is a multiple of 4
         const float4 t = *reinterpret_cast<const float4*>(p + (k < K ? k : 0));
         r.v[4 * q] = t.x; r.v[4 * q + 1] = t.y; r.v[4 * q + 2] = t.z; r.v[4 * q + 3] = t.w;
       } else {
@@ -88,9 +90,15 @@ __device__ __forceinline__ void load_x(const X* p, int s, int g, int K, XRaw<X>&
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int k = 64 * s + 32 * q + 8 * g;
-      if constexpr (WIDE) {   // K is a multiple of 8
+      if constexpr (V == 8) {   // K is a multiple of 8
         const uint4 t = *reinterpret_cast<const uint4*>(p + (k < K ? k : 0));
         r.v[4 * q] = t.x; r.v[4 * q + 1] = t.y; r.v[4 * q + 2] = t.z; r.v[4 * q + 3] = t.w;
+      } else if constexpr (V == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const uint2 t = *reinterpret_cast<const uint2*>(p + (k + e < K ? k + e : 0));
+          r.v[4 * q + e / 2] = t.x; r.v[4 * q + e / 2 + 1] = t.y;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e += 2)
@@ -128,7 +136,7 @@ __device__ __forceinline__ void values_of(const XRaw<X>& r, int s, int g, int K,
 template <typename X>
 constexpr int rows_waves(int ks) { return ks == 8 || ks * sizeof(X) * 4 > 48 ? 2 : 4; }
 
-template <typename X, typename Y, int KS, bool WIDE>
+template <typename X, typename Y, int KS, int V>
 __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8_rows(I8Args a, int slice) {
   extern __shared__ __align__(16) char lds[];
   constexpr int PITCH = KS * 64 + 16;   // 16 bytes more: eight consecutive rows start in different banks
@@ -154,7 +162,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
     asm volatile("" : "+v"(from));   // the column offsets are formed anew per tile: kept, they would not fit the registers
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      if (s < steps) load_x<X, WIDE>(x + row * a.ldx, s, from, a.K, raw[s]);
+      if (s < steps) load_x<X, V>(x + row * a.ldx, s, from, a.K, raw[s]);
   };
   if (tile < tiles) fetch(tile);
 
@@ -247,7 +255,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
       } else {
         patch.put(i, chunk, v);
       }
-      if ((b & 32) || b + 32 >= m_pad) patch.leave(a.y, a.ldy, a.N, 16 * tile, m_begin + (b & ~63), m_begin + m_count, a.wide_out);
+      if ((b & 32) || b + 32 >= m_pad) patch.leave(a.y, a.ldy, a.N, 16 * tile, m_begin + (b & ~63), m_begin + m_count, a.width);
     }
   }
 }
@@ -408,7 +416,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
         }
         patch.put(i32, half * (32 / VEC) + c, v);
       }
-      patch.leave(a.y, a.ldy, a.N, n0 + (wn * TN + j) * 32, mw, a.M, a.wide_out);
+      patch.leave(a.y, a.ldy, a.N, n0 + (wn * TN + j) * 32, mw, a.M, a.width);
     }
   }
 }
@@ -429,7 +437,7 @@ bool i8_by_rows(int64_t N, int K, int M) {
   return ks < 8 ? bytes <= 2 * kI8RowsLds || N <= 4096 : bytes <= kI8RowsLds || N <= 32;
 }
 
-template <typename X, typename Y, int KS, bool WIDE>
+template <typename X, typename Y, int KS, int V>
 int32_t launch_rows(const I8Args& a, hipStream_t stream) {
   const int m32 = (a.M + 31) / 32, per32 = rows_per32(KS);
   const int64_t row_blocks = (a.N + 127) / 128;     // 8 waves of 16 rows
@@ -446,19 +454,19 @@ int32_t launch_rows(const I8Args& a, hipStream_t stream) {
   if (blocks < 1) blocks = 1;
   if (blocks > row_blocks) blocks = row_blocks;
   if (bytes > 64 * 1024)
-    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_rows<X, Y, KS, WIDE>),
+    MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_rows<X, Y, KS, V>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  k_linear_i8_rows<X, Y, KS, WIDE><<<dim3((unsigned)blocks, slices), kI8RowsThreads, bytes, stream>>>(a, per * 32);
+  k_linear_i8_rows<X, Y, KS, V><<<dim3((unsigned)blocks, slices), kI8RowsThreads, bytes, stream>>>(a, per * 32);
   MPNN_LAUNCH_CHECK("k_linear_i8_rows");
   return MPNN_OK;
 }
 
-template <typename X, typename Y, bool WIDE>
+template <typename X, typename Y, int V>
 int32_t rows_of(const I8Args& a, hipStream_t stream) {
-  if (a.K <= 64) return launch_rows<X, Y, 1, WIDE>(a, stream);
-  if (a.K <= 128) return launch_rows<X, Y, 2, WIDE>(a, stream);
-  if (a.K <= 256) return launch_rows<X, Y, 4, WIDE>(a, stream);
-  return launch_rows<X, Y, 8, WIDE>(a, stream);
+  if (a.K <= 64) return launch_rows<X, Y, 1, V>(a, stream);
+  if (a.K <= 128) return launch_rows<X, Y, 2, V>(a, stream);
+  if (a.K <= 256) return launch_rows<X, Y, 4, V>(a, stream);
+  return launch_rows<X, Y, 8, V>(a, stream);
 }
 
 template <typename Y, int WN, int WM, int TN, int PC>
@@ -484,11 +492,12 @@ int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
 }
 
 template <typename Y>
-int32_t launch_i8(const I8Args& a, bool rows, int x_dtype, bool wide_in, hipStream_t stream) {
+int32_t launch_i8(const I8Args& a, bool rows, int x_dtype, int vec_in, hipStream_t stream) {
   if (rows) {
-    if (x_dtype == MPNN_I8) return rows_of<int8_t, Y, true>(a, stream);
-    if (x_dtype == MPNN_F32) return wide_in ? rows_of<float, Y, true>(a, stream) : rows_of<float, Y, false>(a, stream);
-    return wide_in ? rows_of<bf16_t, Y, true>(a, stream) : rows_of<bf16_t, Y, false>(a, stream);
+    if (x_dtype == MPNN_I8) return rows_of<int8_t, Y, 16>(a, stream);
+    if (x_dtype == MPNN_F32) return vec_in == 4 ? rows_of<float, Y, 4>(a, stream) : rows_of<float, Y, 1>(a, stream);
+    if (vec_in == 8) return rows_of<bf16_t, Y, 8>(a, stream);
+    return vec_in == 4 ? rows_of<bf16_t, Y, 4>(a, stream) : rows_of<bf16_t, Y, 1>(a, stream);
   }
   // Tiles of 256 x 256 where they fill the CUs (16,384 rows of 500 -> 1024, 256 tiles: 30 us, with tiles of 128 x 128 32) and
   // are not half empty; of 128 x 128 otherwise (16,384 of 512 -> 512, 128 large tiles: 18 us against 23; 65,536 of 2048 -> 64:
@@ -525,9 +534,8 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: null pointer argument");
   if (((uintptr_t)W & 15) || (ldw & 15) || (x_dtype == MPNN_I8 && (((uintptr_t)X & 15) || (ldx & 15))) || ((uintptr_t)workspace & 15))
     return fail(MPNN_E_INVALID, "mpnn_linear_int8: 8-bit rows and the workspace must be 16-byte aligned");
-  const int vec = y_dtype == MPNN_BF16 ? 8 : 4;
-  const int wide_out = ((uintptr_t)Y & 15) == 0 && ldy % vec == 0;
-  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, wide_out};
+  const int width = store_width(Y, ldy * (y_dtype == MPNN_BF16 ? 2 : 4));
+  I8Args a{X, ldx, x_scale, static_cast<const int8_t*>(W), ldw, w_scale, bias, Y, ldy, N, K, M, relu, width};
   if (take) {
     int8_t* q = static_cast<int8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + N * Kp);
@@ -535,10 +543,11 @@ int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const floa
     if (rc != MPNN_OK) return rc;
     a.x = q; a.ldx = Kp; a.xs = s;
   }
-  const int xvec = x_dtype == MPNN_BF16 ? 8 : 4;
-  const bool wide_in = K % xvec == 0 && ldx % xvec == 0 && ((uintptr_t)X & 15) == 0;
-  return y_dtype == MPNN_BF16 ? launch_i8<bf16_t>(a, rows, x_dtype, wide_in, stream)
-                              : launch_i8<float>(a, rows, x_dtype, wide_in, stream);
+  int vec_in = x_dtype == MPNN_BF16 ? 8 : 4;
+  auto whole = [&](int v) { return K % v == 0 && ldx % v == 0 && (uintptr_t)X % (v * (x_dtype == MPNN_BF16 ? 2 : 4)) == 0; };
+  while (vec_in > 1 && !whole(vec_in)) vec_in = vec_in == 8 ? 4 : 1;
+  return y_dtype == MPNN_BF16 ? launch_i8<bf16_t>(a, rows, x_dtype, vec_in, stream)
+                              : launch_i8<float>(a, rows, x_dtype, vec_in, stream);
 }
 
 }  // extern "C"

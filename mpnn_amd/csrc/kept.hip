@@ -48,7 +48,8 @@ struct KeptArgs {
   void* y; int64_t ldy;
   uint8_t* bits;                    // optional
   int64_t N;
-  int M, relu, wide_out;
+  int M, relu;
+  int width;                        // of the stores (store_width)
   int across;                       // the weights lie as [K, M]: y = x W (one input, nothing kept: the input gradient)
 };
 
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kKeptThreads, kept_waves(KS1, KS2)) k_kept_lin
         const int c = b + 8 * g;
         if (r0 + i < a.N) a.bits[(r0 + i) * (m_pad >> 3) + (c >> 3)] = c < a.M ? (uint8_t)open : (uint8_t)0;
       }
-      if ((b & 32) || b + 32 >= m_pad) patch.leave(a.y, a.ldy, a.N, r0, b & ~63, a.M, true);
+      if ((b & 32) || b + 32 >= m_pad) patch.leave(a.y, a.ldy, a.N, r0, b & ~63, a.M, 16);
     }
     if (a.a.q) keep_rows<KS1>(raw1, a.a, a.N, r0, patch_base);
     if constexpr (KS2 > 0) keep_rows<KS2>(raw2, a.b, a.N, r0, patch_base);
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(kKeptThreads, 2) k_kept_linear_f32(KeptArgs a,
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) patch.put(i, 4 * h + e, {v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]});
-      patch.leave(a.y, a.ldy, a.N, r0, m_begin + b, m_begin + m_count, a.wide_out);
+      patch.leave(a.y, a.ldy, a.N, r0, m_begin + b, m_begin + m_count, a.width);
     }
   }
 }
@@ -493,7 +494,7 @@ int32_t launch_kept1_f32(const KeptArgs& a, hipStream_t stream) {
 int32_t launch_kept_any(KeptArgs& a, int32_t dtype, hipStream_t stream) {
   const int steps = kept_steps(a.a.K);
   if (dtype == MPNN_F32) {
-    a.wide_out = ((uintptr_t)a.y & 15) == 0 && a.ldy % 4 == 0;
+    a.width = store_width(a.y, a.ldy * 4);
     switch (steps) {
       case 1: return launch_kept1_f32<1>(a, stream);
       case 2: return launch_kept1_f32<2>(a, stream);

@@ -102,28 +102,13 @@ struct RowSum {
   }
 };
 
-// VEC columns of T at a time: 16 bytes in float32, 8 in bfloat16, or one column.
-template <typename T, int VEC>
-struct NormIO : RowIO<T, VEC> {};
-template <>
-struct NormIO<bf16_t, 4> {
-  typedef uint2 Raw;
-  static __device__ __forceinline__ Raw load_raw(const bf16_t* p) { return *reinterpret_cast<const uint2*>(p); }
-  static __device__ __forceinline__ void unpack(const Raw& t, float (&v)[4]) {
-    v[0] = __uint_as_float(t.x << 16); v[1] = __uint_as_float(t.x & 0xffff0000u);
-    v[2] = __uint_as_float(t.y << 16); v[3] = __uint_as_float(t.y & 0xffff0000u);
-  }
-  static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[4]) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-  }
-};
-
-// The columns a lane owns: vector v of NV covers columns (v * LPR + lane) * VEC and the VEC - 1 after it.  Raw: the
-// lane's share of a row as it lies in memory, which a row that is on its way takes less registers for.
+// VEC columns of T at a time: 16 bytes in float32, 8 in bfloat16, or one column.  The columns a lane owns: vector v of NV
+// covers columns (v * LPR + lane) * VEC and the VEC - 1 after it.  Raw: the lane's share of a row as it lies in memory,
+// which a row that is on its way takes less registers for.
 template <typename T, int VEC, int NV, int LPR>
 struct Lane {
   static constexpr int C = VEC * NV;
-  typedef NormIO<T, VEC> IO;
+  typedef RowIO<T, VEC> IO;
   struct Raw { typename IO::Raw v[NV]; };
   int col[NV];
   bool in[NV];

@@ -92,6 +92,20 @@ struct RowIO<bf16_t, 8> {
 };
 
 template <>
+struct RowIO<bf16_t, 4> {
+  typedef uint2 Raw;
+  static __device__ __forceinline__ Raw load_raw(const bf16_t* p) { return *reinterpret_cast<const uint2*>(p); }
+  static __device__ __forceinline__ void unpack(const Raw& t, float (&v)[4]) {
+    v[0] = __uint_as_float(t.x << 16); v[1] = __uint_as_float(t.x & 0xffff0000u);
+    v[2] = __uint_as_float(t.y << 16); v[3] = __uint_as_float(t.y & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void load(const bf16_t* p, float (&v)[4]) { unpack(load_raw(p), v); }
+  static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+  }
+};
+
+template <>
 struct RowIO<bf16_t, 1> {
   typedef bf16_t Raw;
   static __device__ __forceinline__ Raw load_raw(const bf16_t* p) { return *p; }

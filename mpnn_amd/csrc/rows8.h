@@ -5,6 +5,7 @@
 namespace mpnn {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
 
 // What a row's largest magnitude (as the bits of a float: infinities and NaN compare above every finite one) makes of it.
 struct Quant {
@@ -66,6 +67,12 @@ __device__ __forceinline__ void store_chunk(void* p, i32x4 v, bool whole) {
   }
 }
 
+// The widest stores that rows `pitch` bytes apart allow: 16 bytes, 8, or one output (0).  1 M x 100 bfloat16 results
+// from 128 columns: 116 us with 8, 207 output by output.
+inline int store_width(const void* y, int64_t pitch) {
+  return ((uintptr_t)y | (uintptr_t)pitch) % 16 == 0 ? 16 : ((uintptr_t)y | (uintptr_t)pitch) % 8 == 0 ? 8 : 0;
+}
+
 // Results of a wave on their way to memory: ROWS rows x COLS outputs in LDS, from where whole row segments leave (128 bytes
 // in bfloat16, 256 in float32; stores of 64 bytes per row took 1.65 instead of 1.20 ms for 4 M rows of 256 in float32).
 // 16-byte chunk c of row r lies at c ^ r (mod the chunks of a row): writes by column and reads by row both spread.  Only
@@ -77,8 +84,9 @@ struct Patch {
   __device__ __forceinline__ void put(int row, int chunk, const float (&v)[VEC]) const {
     store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (COLS * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
   }
-  // To rows r0 .. of y [N, ldy], outputs m .. m + COLS - 1 of which those below `end` exist; wide: 16-byte stores are possible.
-  __device__ __forceinline__ void leave(void* y, int64_t ldy, int64_t N, int64_t r0, int m, int end, bool wide) const {
+  // To rows r0 .. of y [N, ldy], outputs m .. m + COLS - 1 of which those below `end` exist, `width` bytes at a time (see
+  // store_width).
+  __device__ __forceinline__ void leave(void* y, int64_t ldy, int64_t N, int64_t r0, int m, int end, int width) const {
     const int lane = threadIdx.x & 63;
     const bool whole = (ldy * sizeof(Y)) % 64 == 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -90,15 +98,22 @@ struct Patch {
       const int left = end - m - chunk * VEC;
       if (r0 + r >= N || left <= 0) continue;
       Y* const p = static_cast<Y*>(y) + (r0 + r) * ldy + m + chunk * VEC;
-      if (wide && left >= VEC) {
+      if (width == 16 && left >= VEC) {
         store_chunk(p, v, whole);
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (e < left) {
-            if constexpr (sizeof(Y) == 4) p[e] = __uint_as_float((uint32_t)v[e]);
-            else p[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
+        for (int h = 0; h < 2; ++h) {
+          if (width >= 8 && left >= (h + 1) * (VEC / 2)) {
+            *reinterpret_cast<i32x2*>(p + h * (VEC / 2)) = (i32x2){v[2 * h], v[2 * h + 1]};
+          } else {
+#pragma unroll
+            for (int e = h * (VEC / 2); e < (h + 1) * (VEC / 2); ++e)
+              if (e < left) {
+                if constexpr (sizeof(Y) == 4) p[e] = __uint_as_float((uint32_t)v[e]);
+                else p[e] = (Y)((uint32_t)v[e / 2] >> (16 * (e & 1)));
+              }
           }
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -164,11 +164,14 @@ int32_t mpnn_quantize_rows(const void* x, int64_t ldx, int32_t dtype, int64_t N,
   if (!x || !q || !scale) return fail(MPNN_E_INVALID, "mpnn_quantize_rows: null pointer argument");
   if ((uintptr_t)q & 15) return fail(MPNN_E_INVALID, "mpnn_quantize_rows: q must be 16-byte aligned");
   const QuantArgs a{x, ldx, static_cast<int8_t*>(q), ldq, scale, N, K, Kp};
-  const int vec = dtype == MPNN_BF16 ? 8 : 4;
-  // whole 16-byte vectors when width, address and stride allow it, one column per lane and step otherwise
-  const bool wide = K % vec == 0 && ldx % vec == 0 && ((uintptr_t)x & 15) == 0;
-  const bool known = dtype == MPNN_BF16 ? (wide ? launch_quantize<bf16_t, 8>(a, stream) : launch_quantize<bf16_t, 1>(a, stream))
-                                        : (wide ? launch_quantize<float, 4>(a, stream) : launch_quantize<float, 1>(a, stream));
+  // the widest vectors that width, address and stride allow, one column per lane and step otherwise (1 M bfloat16 rows of
+  // 100: 74 us in vectors of 4, 171 by columns)
+  const bool bf16 = dtype == MPNN_BF16;
+  auto whole = [&](int v) { return K % v == 0 && ldx % v == 0 && (uintptr_t)x % (v * (bf16 ? 2 : 4)) == 0; };
+  bool known;
+  if (!bf16) known = whole(4) ? launch_quantize<float, 4>(a, stream) : launch_quantize<float, 1>(a, stream);
+  else if (whole(8)) known = launch_quantize<bf16_t, 8>(a, stream);
+  else known = whole(4) ? launch_quantize<bf16_t, 4>(a, stream) : launch_quantize<bf16_t, 1>(a, stream);
   if (!known) return fail(MPNN_E_INVALID, "mpnn_quantize_rows: no kernel for K=%d", K);
   MPNN_LAUNCH_CHECK("k_quantize_rows");
   return MPNN_OK;

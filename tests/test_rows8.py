@@ -748,3 +748,23 @@ def test_gemm_nn_refuses_before_any_launch():
                 dict(dt=1, ldx=68), dict(dt=1, m=36), dict(k=128, ldx=128, m=4096, ldw=4096, ldy=4096)):
         assert call(**bad) == -1, bad
     assert call(n=0) == 0 and call(n=0, dt=1) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,m", [(300, 100, 100), (65, 500, 36), (33, 4, 12), (200, 252, 50), (300, 600, 300), (513, 1020, 1004)])
+@pytest.mark.parametrize("first", [0, 4, 2])
+def test_rows_on_8_byte_boundaries(n, k, m, first):
+    """Widths and addresses that allow 8 bytes at a time but not 16 (and, first = 2, neither in bfloat16)."""
+    from mpnn_amd import linear_int8, quantize_rows
+    w, b = randn(m, k, seed=m), randn(m, seed=k)
+    wq, ws = quantized(w)
+    w8 = quantize_rows(w.cuda())
+    for dtype in (torch.float32, torch.bfloat16):
+        wider = torch.full((n, k + 8), float("nan"), dtype=dtype)
+        wider[:, first:first + k] = randn(n, k, seed=n).to(dtype)
+        x = wider.cuda()[:, first:first + k]
+        q, s = quantized(wider[:, first:first + k])
+        same_rows(quantize_rows(x), x)
+        for out in (torch.float32, torch.bfloat16):
+            want, bound = linear_reference(q, s, wq, ws, b.to(out), True)
+            close(linear_int8(x, w8, bias=b.to(out).cuda(), relu=True, dtype=out), want, bound)
