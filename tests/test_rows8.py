@@ -768,3 +768,29 @@ def test_rows_on_8_byte_boundaries(n, k, m, first):
         for out in (torch.float32, torch.bfloat16):
             want, bound = linear_reference(q, s, wq, ws, b.to(out), True)
             close(linear_int8(x, w8, bias=b.to(out).cuda(), relu=True, dtype=out), want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_kept_calls_without_rows_with_one_input_twice_and_a_transposed_weight(dtype):
+    from mpnn_amd.dense import project, update
+    wt, wot = randn(64, 32, seed=1, dtype=dtype).cuda(), randn(128, 32, seed=2, dtype=dtype).cuda()
+    for n in (0, 1, 500):
+        x = randn(n, 64, seed=3, dtype=dtype).cuda().requires_grad_()
+        for f, w in ((lambda w: project(x, w, checkpoint="int8"), wt), (lambda w: update(x, x, w, checkpoint="int8"), wot)):
+            got = []
+            for v in (w.t(), w.t().contiguous()):                     # [32, 64], [32, 128]
+                v = v.detach().requires_grad_()
+                y = f(v)
+                assert y.shape == (n, 32)
+                got.append((y.detach(), *torch.autograd.grad(y, (x, v), torch.ones_like(y))))
+            # a transposed weight takes the general product, whose sums may run in another order: some 10 units in size here, each
+            # off by at most 128 * 2^-24 of 64, and one rounding to the type
+            for p, q in zip(*got):
+                assert bool(((p.double() - q.double()).abs() <= 4 * torch.finfo(dtype).eps * (q.double().abs() + 64)).all())
+            assert n > 0 or not got[0][2].any()
+        y = update(x, x, wot.t().contiguous().requires_grad_(), checkpoint="int8")
+        (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        z = [x.detach().clone().requires_grad_() for _ in range(2)]
+        ga, gb = torch.autograd.grad(update(z[0], z[1], wot.t().contiguous().requires_grad_(), checkpoint="int8"), z, torch.ones_like(y))
+        assert torch.equal(gx, ga + gb)
