@@ -41,7 +41,7 @@ enum {
   MPNN_E_CAPACITY = -4   /* an output array's stated capacity is too small */
 };
 
-#define MPNN_ABI_VERSION 22
+#define MPNN_ABI_VERSION 23
 
 /* Library self-description. */
 int32_t mpnn_abi_version(void);
@@ -655,6 +655,8 @@ int32_t mpnn_quantize_rows(const void* X, int64_t ldx, int32_t dtype, int64_t N,
 int32_t mpnn_relu_bits(const void* Y, int64_t ldy, int32_t dtype, int64_t N, int32_t M, void* bits,
                        mpnn_stream_t stream);
 int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_t x_dtype);
+/* LDS bytes a block of mpnn_linear_int8's kernel takes for these sizes (at most the 160 KiB of a CU); -1: sizes it refuses. */
+int64_t mpnn_linear_int8_lds_bytes(int64_t N, int32_t K, int32_t M, int32_t y_dtype);
 int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const float* x_scale, const void* W, int64_t ldw,
                          const float* w_scale, const void* bias, void* Y, int64_t ldy, int32_t y_dtype, int64_t N,
                          int32_t K, int32_t M, int32_t relu, void* workspace, mpnn_stream_t stream);

@@ -15,7 +15,7 @@ MPNN_F32 = 0
 MPNN_BF16 = 1
 MPNN_U8 = 2
 MPNN_I8 = 3
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 LIB_PATH = os.environ.get("MPNN_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmpnn_amd.so")
 
@@ -162,6 +162,7 @@ SIGNATURES = {
     "mpnn_quantize_rows": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
     "mpnn_relu_bits": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p]),
     "mpnn_linear_int8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    "mpnn_linear_int8_lds_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
     "mpnn_linear_int8": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                    c_int64, c_int32, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "mpnn_kept_linear_fits": (c_int32, [c_int32, c_int32, c_int32, c_int32]),

@@ -422,6 +422,9 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
 }
 
 // --------------------------------------------------------------------------------------------------------- dispatch
+// Steps of 64 columns of a width, as the rows kernel comes.
+int rows_steps(int K) { return K <= 64 ? 1 : K <= 128 ? 2 : K <= 256 ? 4 : 8; }
+
 // LDS bytes of 32 output columns in the rows kernel: weights, scales, biases.
 constexpr int rows_per32(int ks) { return 32 * (ks * 64 + 16 + 8); }
 
@@ -432,41 +435,56 @@ constexpr int rows_per32(int ks) { return 32 * (ks * 64 + 16 + 8); }
 // rows (512 -> 2048: 7.7 against 10.0 us for 18), and loses with more (65,536 rows of 512 -> 512, three slices: 69 against 49).
 bool i8_by_rows(int64_t N, int K, int M) {
   if (K > 512) return false;
-  const int ks = K <= 64 ? 1 : K <= 128 ? 2 : K <= 256 ? 4 : 8;
+  const int ks = rows_steps(K);
   const int64_t bytes = (int64_t)((M + 31) / 32) * rows_per32(ks);
   return ks < 8 ? bytes <= 2 * kI8RowsLds || N <= 4096 : bytes <= kI8RowsLds || N <= 32;
 }
 
-template <typename X, typename Y, int KS, int V>
-int32_t launch_rows(const I8Args& a, hipStream_t stream) {
-  const int m32 = (a.M + 31) / 32, per32 = rows_per32(KS);
-  const int64_t row_blocks = (a.N + 127) / 128;     // 8 waves of 16 rows
-  // weights: as few slices as fit, more of them when the rows alone would leave CUs without work
+// What a launch of the rows kernel asks for: groups of 32 outputs per slice, slices, and LDS bytes of a block.
+struct RowsPlan { int per, slices, bytes; };
+constexpr int kI8Lds = 160 * 1024;       // of a CU
+
+template <typename Y>
+RowsPlan rows_plan(int64_t N, int M, int ks) {
+  constexpr int patches = kI8RowsThreads / 64 * (int)Patch<Y, 16>::BYTES;
+  const int m32 = (M + 31) / 32, per32 = rows_per32(ks);
+  const int most = (kI8Lds - patches) / per32;      // groups of a slice that fit next to the result patches
+  const int64_t row_blocks = (N + 127) / 128;       // 8 waves of 16 rows
+  // as few slices as fit the room for weights, more of them when the rows alone would leave CUs without work
   int slices = (m32 * per32 + kI8RowsLds - 1) / kI8RowsLds;
   while (slices < m32 && row_blocks * slices < 256) ++slices;
   int per = (m32 + slices - 1) / slices;
+  if (per > most) per = most;                       // (the share was rounded up to whole groups)
   slices = (m32 + per - 1) / per;
-  const int bytes = per * per32 + kI8RowsThreads / 64 * (int)Patch<Y, 16>::BYTES;
-  int per_cu = 160 * 1024 / bytes;
+  return RowsPlan{per, slices, per * per32 + patches};
+}
+
+template <typename X, typename Y, int KS, int V>
+int32_t launch_rows(const I8Args& a, hipStream_t stream) {
+  const RowsPlan p = rows_plan<Y>(a.N, a.M, KS);
+  const int64_t row_blocks = (a.N + 127) / 128;
+  int per_cu = kI8Lds / p.bytes;
   const int by_regs = rows_waves<X>(KS) / 2;
   if (per_cu > by_regs) per_cu = by_regs;
-  int64_t blocks = 256 * per_cu / slices;
+  int64_t blocks = 256 * per_cu / p.slices;
   if (blocks < 1) blocks = 1;
   if (blocks > row_blocks) blocks = row_blocks;
-  if (bytes > 64 * 1024)
+  if (p.bytes > 64 * 1024)
     MPNN_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear_i8_rows<X, Y, KS, V>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  k_linear_i8_rows<X, Y, KS, V><<<dim3((unsigned)blocks, slices), kI8RowsThreads, bytes, stream>>>(a, per * 32);
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, p.bytes));
+  k_linear_i8_rows<X, Y, KS, V><<<dim3((unsigned)blocks, p.slices), kI8RowsThreads, p.bytes, stream>>>(a, p.per * 32);
   MPNN_LAUNCH_CHECK("k_linear_i8_rows");
   return MPNN_OK;
 }
 
 template <typename X, typename Y, int V>
 int32_t rows_of(const I8Args& a, hipStream_t stream) {
-  if (a.K <= 64) return launch_rows<X, Y, 1, V>(a, stream);
-  if (a.K <= 128) return launch_rows<X, Y, 2, V>(a, stream);
-  if (a.K <= 256) return launch_rows<X, Y, 4, V>(a, stream);
-  return launch_rows<X, Y, 8, V>(a, stream);
+  switch (rows_steps(a.K)) {
+    case 1: return launch_rows<X, Y, 1, V>(a, stream);
+    case 2: return launch_rows<X, Y, 2, V>(a, stream);
+    case 4: return launch_rows<X, Y, 4, V>(a, stream);
+    default: return launch_rows<X, Y, 8, V>(a, stream);
+  }
 }
 
 template <typename Y, int WN, int WM, int TN, int PC>
@@ -491,6 +509,11 @@ int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
   return MPNN_OK;
 }
 
+// Tiles of 256 x 256 where they fill the CUs (16,384 rows of 500 -> 1024, 256 tiles: 30 us, with tiles of 128 x 128 32) and
+// are not half empty; of 128 x 128 otherwise (16,384 of 512 -> 512, 128 large tiles: 18 us against 23; 65,536 of 2048 -> 64:
+// 103 against 112).
+bool i8_large_tiles(int64_t N, int M) { return M > 128 && ((N + 255) / 256) * ((M + 255) / 256) >= 256; }
+
 template <typename Y>
 int32_t launch_i8(const I8Args& a, bool rows, int x_dtype, int vec_in, hipStream_t stream) {
   if (rows) {
@@ -499,11 +522,7 @@ int32_t launch_i8(const I8Args& a, bool rows, int x_dtype, int vec_in, hipStream
     if (vec_in == 8) return rows_of<bf16_t, Y, 8>(a, stream);
     return vec_in == 4 ? rows_of<bf16_t, Y, 4>(a, stream) : rows_of<bf16_t, Y, 1>(a, stream);
   }
-  // Tiles of 256 x 256 where they fill the CUs (16,384 rows of 500 -> 1024, 256 tiles: 30 us, with tiles of 128 x 128 32) and
-  // are not half empty; of 128 x 128 otherwise (16,384 of 512 -> 512, 128 large tiles: 18 us against 23; 65,536 of 2048 -> 64:
-  // 103 against 112).
-  if (a.M > 128 && ((a.N + 255) / 256) * ((a.M + 255) / 256) >= 256) return launch_tiles<Y, 2, 4, 4, 8>(a, stream);
-  return launch_tiles<Y, 2, 2, 2, 8>(a, stream);
+  return i8_large_tiles(a.N, a.M) ? launch_tiles<Y, 2, 4, 4, 8>(a, stream) : launch_tiles<Y, 2, 2, 2, 8>(a, stream);
 }
 
 }  // namespace
@@ -517,6 +536,13 @@ int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_
   if (N < 0 || K < 1 || K > kI8MaxK || M < 1 || M > kI8MaxM) return -1;
   if (x_dtype == MPNN_I8 || i8_by_rows(N, K, M)) return 0;
   return N * ((K + 15) / 16 * 16) + align_up(N * 4, 16);
+}
+
+int64_t mpnn_linear_int8_lds_bytes(int64_t N, int32_t K, int32_t M, int32_t y_dtype) {
+  if (N < 0 || K < 1 || K > kI8MaxK || M < 1 || M > kI8MaxM || (y_dtype != MPNN_F32 && y_dtype != MPNN_BF16)) return -1;
+  if (i8_by_rows(N, K, M))
+    return y_dtype == MPNN_BF16 ? rows_plan<bf16_t>(N, M, rows_steps(K)).bytes : rows_plan<float>(N, M, rows_steps(K)).bytes;
+  return i8_large_tiles(N, M) ? tiles_lds<2, 4, 4, 8>() : tiles_lds<2, 2, 2, 8>();
 }
 
 int32_t mpnn_linear_int8(const void* X, int64_t ldx, int32_t x_dtype, const float* x_scale, const void* W, int64_t ldw,

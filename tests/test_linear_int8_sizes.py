@@ -1,0 +1,47 @@
+"""linear_int8 over its whole documented range of sizes: the plan of every launch fits a CU's LDS, and the widest heads answer a
+few rows."""
+import pytest
+import torch
+
+from mpnn_amd import _lib
+
+U = 2.0 ** -24
+
+
+def test_every_plan_fits_the_lds_of_a_cu():
+    """On the host: every number of outputs up to 2^20 in steps of 32 (and one above), every form of the kernels."""
+    size = _lib.load().mpnn_linear_int8_lds_bytes
+    most = 160 * 1024
+    for k in (64, 128, 256, 300, 512, 513, 8192):
+        for n in (1, 32, 33, 100, 4096, 4097, 1000000):
+            for out in (_lib.MPNN_F32, _lib.MPNN_BF16):
+                worst = max(size(n, k, m, out) for m in range(32, (1 << 20) + 1, 32))
+                assert 0 < worst <= most, (k, n, out, worst)
+                assert size(n, k, 57345, out) <= most and size(n, k, 1, out) > 0
+    for bad in ((-1, 8, 8, 0), (1, 0, 8, 0), (1, 8193, 8, 0), (1, 8, 0, 0), (1, 8, (1 << 20) + 1, 0), (1, 8, 8, 2)):
+        assert size(*bad) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 32])
+@pytest.mark.parametrize("k", [300, 512])
+@pytest.mark.parametrize("m", [57344, 57345, 128256])
+def test_few_rows_against_a_wide_head(n, k, m):
+    """Sums of whole numbers are exact; the scales, their application and the bias round once each."""
+    from mpnn_amd import linear_int8, quantize_rows
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    x, w = (torch.randn(r, k, generator=gen, device="cuda") for r in (n, m))
+    b = torch.randn(m, generator=gen, device="cuda")
+    xr, wr = quantize_rows(x), quantize_rows(w)
+    exact = (xr.values.double() @ wr.values.double().t()) * (xr.scale.double().unsqueeze(1) * wr.scale.double())
+    for out in (torch.float32, torch.bfloat16):
+        bias = b.to(out)
+        want = exact + bias.double()
+        bound = 3 * U * exact.abs() + U * want.abs()
+        bound = bound + torch.finfo(out).eps / 2 * (want.abs() + bound)
+        first = None
+        for rows in (x, xr):
+            got = linear_int8(rows, wr, bias=bias, dtype=out)
+            assert got.shape == (n, m) and bool(((got.double() - want).abs() <= bound).all())
+            first = got if first is None else first
+            assert torch.equal(got, first)
