@@ -60,4 +60,10 @@ struct Arena {
 constexpr int kBlock = 256;
 constexpr int kMaxBlocks = 2048;
 
+// The calling wave's copies from memory straight to LDS (global_load_lds) have landed.  Stands before the barrier that
+// publishes them to the block: a barrier by itself orders LDS accesses only, and the compiler adds the wait for the copies to it
+// in most kernels but not in all - a form of k_linear_i8_tiles with spilled registers was built without it in its loop, and read
+// rows that were still on their way now and then.
+__device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 }  // namespace mpnn

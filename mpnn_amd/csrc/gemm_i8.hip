@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
   const int wn = wave / WM, wm = wave % WM;
   // Blocks stay and go round the tiles, those of one XCD (block index mod 8) through all column tiles of a row tile one
   // after the other, so that a row tile is fetched into one L2 only.  A tile's last step already copies the next tile's
-  // first, and its results leave while that is on its way.
+  // first, under its products; the barrier before the results waits for that copy.
   const int xcd = blockIdx.x & 7, turn = gridDim.x >> 3;
   const int Kp = (a.K + 15) & ~15, pieces = Kp >> 4;
 
@@ -336,9 +336,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
     const int64_t n0 = (int64_t)((tile / m_tiles) * 8 + xcd) * BN;
     const int m0 = tile % m_tiles * BM;
     tile += turn;
-    // What the results need besides the sums is loaded here, ahead of a barrier that waits for everything.  While copies
-    // to LDS are on their way nothing is loaded into registers and nothing may be spilled: values that were reloaded
-    // under them came out wrong now and then.
+    // what the results need besides the sums, ahead of a wait that is due anyway
     float xs[TN], ws = 0.f, bs = 0.f;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -358,7 +356,8 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[j][t][r] = 0;
     for (int p0 = 0; p0 < pieces; p0 += PC, buf ^= 1) {
-      __syncthreads();                     // this step's copies have landed, the other buffer is read no more
+      copies_landed();
+      __syncthreads();                     // this step's rows are here, the other buffer is read no more
       if (p0 + PC < pieces) stage(buf ^ 1, p0 + PC);
       else if ((more = take(tile))) stage(buf ^ 1, 0);
       const char* const xb = lds + buf * STAGE + (wn * TN * 32 + i32) * ROW;
@@ -368,6 +367,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
           i32x4* const p = reinterpret_cast<i32x4*>(lds + buf * STAGE + r * ROW + piece_at<PC>(r, pieces - 1 - p0) * 16);
           *p = keep_bytes(*p, a.K & 15);
         }
+        copies_landed();                   // (no copy is on its way across a barrier)
         __syncthreads();
       }
       i32x4 w[2][2], v[2][TN];                 // the operands of one product are on their way while the one before runs
@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
       s_bs[threadIdx.x] = bs;
     }
     const int mw = m0 + wm * 64;
+    copies_landed();
     __syncthreads();                       // every wave has read its operands: the buffer may take results
     const Patch<Y, 32> patch{lds + (buf ^ 1) * STAGE + wave * (int)Patch<Y, 32>::BYTES};
     constexpr int VEC = Patch<Y, 32>::VEC;
@@ -497,12 +498,6 @@ int32_t launch_tiles(const I8Args& a, hipStream_t stream) {
   const int64_t grid = all < resident ? all : resident;
   if (all > INT32_MAX) return fail(MPNN_E_INVALID, "mpnn_linear_int8: N=%lld M=%d", (long long)a.N, a.M);
   const void* const f = reinterpret_cast<const void*>(k_linear_i8_tiles<Y, WN, WM, TN, PC>);
-  static const hipError_t sound = [f] {   // a build that had to spill registers is not run (see the kernel)
-    hipFuncAttributes attr;
-    const hipError_t e = hipFuncGetAttributes(&attr, f);
-    return e != hipSuccess ? e : (attr.localSizeBytes != 0 ? hipErrorInvalidKernelFile : hipSuccess);
-  }();
-  MPNN_HIP_CHECK(sound);
   MPNN_HIP_CHECK(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
   k_linear_i8_tiles<Y, WN, WM, TN, PC><<<(unsigned)grid, WN * WM * 64, bytes, stream>>>(a, (int)nt, (int)mt);
   MPNN_LAUNCH_CHECK("k_linear_i8_tiles");
