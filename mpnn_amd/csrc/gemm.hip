@@ -823,8 +823,8 @@ __global__ void __launch_bounds__(512, 1) k_gemm_nt_ws(NtArgs a) {
       }
   };
   // The weight images go from global memory straight into LDS (no registers): every consumer wave copies its share
-  // of the 1-KiB pieces of chunk i + 2 at the start of iteration i, and the barrier at the end of the iteration
-  // (whose fence waits for the copies) publishes them; they are first read in iteration i + 1.
+  // of the 1-KiB pieces of chunk i + 2 at the start of iteration i, waits for them at its end, and the barrier there
+  // publishes them; they are first read in iteration i + 1.
   int w_c = 2 % nch;   // chunk of the next image to copy
   auto copy_w = [&](int c, int stage) __attribute__((always_inline)) {
     const char* img = a.wimg + ((int64_t)blockIdx.y * nch + c) * WIMG + lane * 16;
@@ -839,6 +839,7 @@ __global__ void __launch_bounds__(512, 1) k_gemm_nt_ws(NtArgs a) {
   };
   copy_w(0, 0);
   copy_w(1 % nch, 1);
+  copies_landed();
   WS_SYNC();
   read_a(0, ldsb);
   read_a(1, ldsb);
@@ -885,6 +886,7 @@ __global__ void __launch_bounds__(512, 1) k_gemm_nt_ws(NtArgs a) {
       epilogue();
 #endif
     }
+    copies_landed();
     WS_SYNC();
   }
 #ifdef MPNN_WS_PROF
