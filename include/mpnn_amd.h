@@ -639,9 +639,10 @@ int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
  * mpnn_quantize_rows    X [N, K] (dtype, any row stride) -> Q [N, ldq] (16-byte aligned, ldq a multiple of 16; the
  *   bytes behind K are written as zeros), scale [N].  1 <= K <= 8192.
  * mpnn_relu_bits        bits [N][ceil(M / 32)] words: bit i of word w is set unless Y[n, 32 w + i] <= 0.
- * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * (x_scale[n] * w_scale[m]) + bias[m]); the sum is exact.  x_dtype
- *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits first, in the
- *   workspace (mpnn_linear_int8_workspace_bytes, 16-byte aligned).  W [M, ldw] 8-bit rows with w_scale [M]; bias [M]
+ * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * x_scale[n] * w_scale[m] + bias[m]); the sum is exact, the scales
+ *   follow in float32 in the order that stays in its range (x_scale first where it is at most 1, else last).  x_dtype
+ *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits first, in the workspace
+ *   (mpnn_linear_int8_workspace_bytes, 16-byte aligned).  W [M, ldw] 8-bit rows with w_scale [M]; bias [M]
  *   of y_dtype or NULL.  8-bit rows 16-byte aligned, strides multiples of 16 and (mpnn_linear_int8) at most
  *   2^22; K <= 8192, M <= 2^20.
  * mpnn_gemm_tn8         dW[M, K + K2] = sum_n (G * open)[n, :]^T [scale[n] Q[n, :] | scale2[n] Q2[n, :]]

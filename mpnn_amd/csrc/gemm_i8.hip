@@ -1,6 +1,6 @@
 // Product of 8-bit rows with 8-bit weights (rows8.hip holds the format):
 //
-//   y[n, m] = act( (sum_k xq[n, k] * wq[m, k]) * (xs[n] * ws[m]) + bias[m] )
+//   y[n, m] = act( (sum_k xq[n, k] * wq[m, k]) * xs[n] * ws[m] + bias[m] )
 //
 // the forward of a Linear call (models/layers.py:104,140, models/mpnn.py:101) of a trained model, with one scale per
 // row of x and one per output channel.  The sum is exact (32-bit integers: 127 * 127 * K stays below 2^31 for
@@ -40,8 +40,17 @@ struct I8Args {
   int width;                       // of the stores (store_width)
 };
 
-__device__ __forceinline__ float finish(int32_t acc, float scale, float bias, int relu) {
-  const float v = fmaf((float)acc, scale, bias);
+// A row's scale, as the factor the sum meets before the weight's scale and the one it meets after it.  The sum is a whole number
+// below 2^28 and scales of rows are at least 2^-107: with a scale of at most 1 first, or one above 1 last, no product on the way
+// leaves float32's range unless the result does (scale times scale would: 2^120 and 2^10 leave no zero of a sum of 0).
+struct RowScale { float before, after; };
+__device__ __forceinline__ RowScale row_scale(float xs) {
+  const bool small = xs <= 1.f;           // a NaN goes last
+  return RowScale{small ? xs : 1.f, small ? 1.f : xs};
+}
+
+__device__ __forceinline__ float finish(int32_t acc, RowScale x, float ws, float bias, int relu) {
+  const float v = fmaf((float)acc * x.before * ws, x.after, bias);
   return relu && v <= 0.f ? 0.f : v;      // a NaN stays
 }
 
@@ -229,6 +238,7 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
         }
     }
     if (tile + step < tiles) fetch(tile + step);
+    const RowScale scale = row_scale(xs);
     for (int b = 0; b < m_pad; b += 32) {
       i32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
       const char* w = lds + (b + i) * PITCH + g * 16;
@@ -243,10 +253,10 @@ __global__ void __launch_bounds__(kI8RowsThreads, rows_waves<X>(KS)) k_linear_i8
       for (int t = 0; t < 2; ++t) {
         const float4 ws = *reinterpret_cast<const float4*>(s_ws + b + 8 * g + 4 * t);
         const float4 bs = *reinterpret_cast<const float4*>(s_bias + b + 8 * g + 4 * t);
-        v[4 * t] = finish(acc[t][0], xs * ws.x, bs.x, a.relu);
-        v[4 * t + 1] = finish(acc[t][1], xs * ws.y, bs.y, a.relu);
-        v[4 * t + 2] = finish(acc[t][2], xs * ws.z, bs.z, a.relu);
-        v[4 * t + 3] = finish(acc[t][3], xs * ws.w, bs.w, a.relu);
+        v[4 * t] = finish(acc[t][0], scale, ws.x, bs.x, a.relu);
+        v[4 * t + 1] = finish(acc[t][1], scale, ws.y, bs.y, a.relu);
+        v[4 * t + 2] = finish(acc[t][2], scale, ws.z, bs.z, a.relu);
+        v[4 * t + 3] = finish(acc[t][3], scale, ws.w, bs.w, a.relu);
       }
       const int chunk = ((b & 32) + 8 * g) / patch.VEC;
       if constexpr (sizeof(Y) == 4) {
@@ -400,6 +410,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
     constexpr int VEC = Patch<Y, 32>::VEC;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
+      const RowScale scale = row_scale(xs[j]);
 #pragma unroll
       for (int c = 0; c < 32 / VEC; ++c) {
         float v[VEC], sw[VEC], sb[VEC];
@@ -413,7 +424,7 @@ __global__ void __launch_bounds__(WN * WM * 64, 2) k_linear_i8_tiles(I8Args a, i
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const int o = c * VEC + e;
-          v[e] = finish(acc[j][o >> 4][o & 15], xs[j] * sw[e], sb[e], a.relu);
+          v[e] = finish(acc[j][o >> 4][o & 15], scale, sw[e], sb[e], a.relu);
         }
         patch.put(i32, half * (32 / VEC) + c, v);
       }

@@ -45,3 +45,28 @@ def test_few_rows_against_a_wide_head(n, k, m):
             assert got.shape == (n, m) and bool(((got.double() - want).abs() <= bound).all())
             first = got if first is None else first
             assert torch.equal(got, first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,m", [(5, 64, 40), (40, 8192, 70)])
+def test_scales_whose_product_leaves_the_range_of_float32(n, k, m):
+    """A sum of zero stays zero where scale times scale would be infinite, and a result inside float32's range keeps its digits where
+    scale times scale would be denormal: what the definition's factors make of it in 64 bits, three roundings off at most."""
+    from mpnn_amd import linear_int8, quantize_rows
+    U = 2.0 ** -24
+    x = torch.zeros(n, k)
+    w = torch.zeros(m, k)
+    x[:, 0], w[:, 1] = 3e38, 1e5                      # disjoint columns: every sum is 0
+    xs, ws = (t[0, c] / 127 for t, c in ((x, 0), (w, 1)))
+    assert not torch.isfinite(xs * ws)
+    b = torch.arange(m).float()
+    assert torch.equal(linear_int8(x.cuda(), quantize_rows(w.cuda()), bias=b.cuda()).cpu(), b.expand(n, m))
+    gen = torch.Generator().manual_seed(m)
+    for up, down in ((2.0 ** -60, 2.0 ** -66), (2.0 ** -66, 2.0 ** -60), (2.0 ** 100, 2.0 ** -100), (2.0 ** -100, 2.0 ** 100),
+                     (2.0 ** 120, 2.0 ** -90), (2.0 ** -90, 2.0 ** 120)):
+        xr = quantize_rows((up * torch.rand(n, k, generator=gen)).cuda())
+        wr = quantize_rows((down * torch.rand(m, k, generator=gen)).cuda())
+        want = (xr.values.double() @ wr.values.double().t()) * xr.scale.double().unsqueeze(1) * wr.scale.double()
+        got = linear_int8(xr, wr).double()
+        # (the smallest step of float32's range, where the result itself lies below it)
+        assert bool(((got - want).abs() <= 3.01 * U * want.abs() + 2.0 ** -149).all()), (up, down)
