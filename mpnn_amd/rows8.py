@@ -124,7 +124,7 @@ def linear_int8(x, weight: Rows8, bias: torch.Tensor | None = None, relu: bool =
     """``act(x @ weight^T + bias)`` on 8-bit rows with exact integer sums: x [N, K] as ``Rows8``, or in float32 / bfloat16
     (taken to 8 bits on the way, one scale per row); ``weight`` [M, K] one scale per output channel, made once with
     ``quantize_rows(w)``.  The result is ``dtype`` (x's own by default, float32 for ``Rows8``); ``bias`` [M] of that dtype.
-    For answering only: no gradient."""
+    For answering only: operands that want a gradient are refused where gradients are recorded."""
     return (_marked_linear if torch.compiler.is_compiling() else _linear_int8)(x, weight, bias, relu, dtype)
 
 
@@ -132,13 +132,14 @@ def _linear_int8(x, weight, bias, relu, dtype):
     held = isinstance(x, Rows8)
     if not isinstance(weight, Rows8):
         raise TypeError(f"weight must be Rows8 (quantize_rows(w)), got {type(weight).__name__}")
+    if torch.is_grad_enabled() and ((x.scale if held else x).requires_grad or weight.scale.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() (or with detached operands), or train "
+                           'with dense.project(..., checkpoint="int8")')
     if held:
         _lib.require_device(x.values, "x")
     else:
         _check_rows("x", x)
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad(), or train with "
-                               'dense.project(..., checkpoint="int8")')
         x = _lib.rows_in_place(x)
     n, k = x.shape
     m = weight.shape[0]

@@ -70,3 +70,17 @@ def test_scales_whose_product_leaves_the_range_of_float32(n, k, m):
         got = linear_int8(xr, wr).double()
         # (the smallest step of float32's range, where the result itself lies below it)
         assert bool(((got - want).abs() <= 3.01 * U * want.abs() + 2.0 ** -149).all()), (up, down)
+
+
+def test_every_operand_that_wants_a_gradient_is_refused():
+    """On the host, before any device is asked for: a bias or a scale whose gradient would be dropped, not x alone."""
+    from mpnn_amd import Rows8, linear_int8
+    rows = lambda n, grad=False: Rows8(torch.zeros(n, 16, dtype=torch.int8), torch.ones(n, requires_grad=grad))
+    x, b = torch.zeros(4, 16), torch.zeros(8)
+    wanted = (((x.clone().requires_grad_(), rows(8)), {}), ((x, rows(8)), dict(bias=b.clone().requires_grad_())), ((x, rows(8, True)), {}),
+              ((rows(4, True), rows(8)), {}), ((rows(4), rows(8)), dict(bias=torch.nn.Parameter(b))))
+    for args, kw in wanted:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            linear_int8(*args, **kw)
+        with torch.no_grad(), pytest.raises(_lib.MpnnError, match="GPU"):      # as far as a host without a GPU gets
+            linear_int8(*args, **kw)
