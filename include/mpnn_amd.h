@@ -41,7 +41,7 @@ enum {
   MPNN_E_CAPACITY = -4   /* an output array's stated capacity is too small */
 };
 
-#define MPNN_ABI_VERSION 23
+#define MPNN_ABI_VERSION 24
 
 /* Library self-description. */
 int32_t mpnn_abi_version(void);
@@ -639,6 +639,8 @@ int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
  * mpnn_quantize_rows    X [N, K] (dtype, any row stride) -> Q [N, ldq] (16-byte aligned, ldq a multiple of 16; the
  *   bytes behind K are written as zeros), scale [N].  1 <= K <= 8192.
  * mpnn_relu_bits        bits [N][ceil(M / 32)] words: bit i of word w is set unless Y[n, 32 w + i] <= 0.
+ * mpnn_open_entries     Gout[n, m] = G[n, m] where bit m of such bits is set, zero elsewhere (the gradient of the relu they came
+ *   from); G and Gout [N, M] of dtype, any row stride.
  * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * x_scale[n] * w_scale[m] + bias[m]); the sum is exact, the scales
  *   follow in float32 in the order that stays in its range (x_scale first where it is at most 1, else last).  x_dtype
  *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits first, in the workspace
@@ -655,6 +657,8 @@ int32_t mpnn_quantize_rows(const void* X, int64_t ldx, int32_t dtype, int64_t N,
                            float* scale, mpnn_stream_t stream);
 int32_t mpnn_relu_bits(const void* Y, int64_t ldy, int32_t dtype, int64_t N, int32_t M, void* bits,
                        mpnn_stream_t stream);
+int32_t mpnn_open_entries(const void* G, int64_t ldg, int32_t dtype, const void* bits, void* Gout, int64_t ldgo, int64_t N,
+                          int32_t M, mpnn_stream_t stream);
 int64_t mpnn_linear_int8_workspace_bytes(int64_t N, int32_t K, int32_t M, int32_t x_dtype);
 /* LDS bytes a block of mpnn_linear_int8's kernel takes for these sizes (at most the 160 KiB of a CU); -1: sizes it refuses. */
 int64_t mpnn_linear_int8_lds_bytes(int64_t N, int32_t K, int32_t M, int32_t y_dtype);

