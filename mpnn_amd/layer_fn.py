@@ -31,7 +31,7 @@ from . import islands, ops
 from .dense import gemm_nt, gemm_nt_bf16, gemm_tn, gemm_tn_bf16
 from .graph import MPGraph
 from .rows8 import MAX_WIDTH as ROWS8_MAX_WIDTH
-from .rows8 import gemm_tn8, kept_linear, relu_bits, rows8_again, to_rows8
+from .rows8 import gemm_tn8, kept_linear, open_entries, relu_bits, rows8_again, to_rows8
 
 
 def fused_x(dtype, f: int, h: int) -> bool:
@@ -203,17 +203,20 @@ class _KeptLayerFn(torch.autograd.Function):
         a, b = ab[:, :h], ab[:, h:]
         ea_s, ea_t = ops._prepare(a, b, edge_attr, w_edge, graph)
         aggr, cnt, maskbits = ops._run_forward(a, b, ea_s, w_edge, graph.by_dst, graph, True)
-        both = kept_linear(x, w_out, aggr, relu=True)
+        # the weight gradients alone read the rows: x's for either weight, aggr's for w_out
+        _, _, need_wn, _, need_wout, _ = ctx.needs_input_grad
+        both = kept_linear(x, w_out, aggr, relu=True) if need_wout else None
         if both is not None:
             y, rx, ra, bits = both
         else:
             y = (gemm_nt_bf16 if bf else gemm_nt)(x, w_out[:, :f], aggr, w_out[:, f:], relu=True)
-            rx, ra, bits = to_rows8(x), to_rows8(aggr), relu_bits(y)
+            rx, ra = to_rows8(x) if need_wn or need_wout else None, to_rows8(aggr) if need_wout else None
+            bits = relu_bits(y)
         if maskbits is not None:
             graph.tpos                       # built once per graph, outside the backward
-        ctx.save_for_backward(rx.values, rx.scale, ra.values, ra.scale, bits, cnt[0], cnt[1], maskbits,
-                              ab if maskbits is None else None, ea_t, w_nodes, w_edge, w_out)
-        ctx.graph = graph
+        rows = [t for r in (rx, ra) for t in ((r.values, r.scale) if r is not None else (None, None))]
+        ctx.save_for_backward(*rows, bits, cnt[0], cnt[1], maskbits, ab if maskbits is None else None, ea_t, w_nodes, w_edge, w_out)
+        ctx.graph, ctx.f = graph, f
         return y
 
     @staticmethod
@@ -221,15 +224,20 @@ class _KeptLayerFn(torch.autograd.Function):
     def backward(ctx, gy):
         xv, xs, av, as_, bits, cnt8, cnt_big, maskbits, ab, ea_t, w_nodes, w_edge, w_out = ctx.saved_tensors
         graph = ctx.graph
+        need_x, _, need_wn, need_we, need_wout, _ = ctx.needs_input_grad
         bf = gy.dtype == torch.bfloat16
         nt = gemm_nt_bf16 if bf else gemm_nt
-        f, h = xv.size(1), w_out.size(0)
-        rx, n = rows8_again(xv, xs), xv.size(0)
+        f, (n, h) = ctx.f, gy.shape
+        rx = rows8_again(xv, xs) if xv is not None else None
         gy = gy.contiguous()
         if gy.data_ptr() % 16:
             gy = gy.clone()
-        gz = torch.empty_like(gy)
-        g_wout = gemm_tn8(gy, rx, rows8_again(av, as_), bits=bits, g_out=gz)
+        g_wout = None
+        if need_wout:
+            gz = torch.empty_like(gy)
+            g_wout = gemm_tn8(gy, rx, rows8_again(av, as_), bits=bits, g_out=gz)
+        else:
+            gz = open_entries(gy, bits)
         wt_out = w_out.t().contiguous()                   # [F+H, H]
         g_ab = torch.empty((n, 2 * h), dtype=gy.dtype, device=gy.device)
         cnt = (cnt8, cnt_big)
@@ -237,9 +245,9 @@ class _KeptLayerFn(torch.autograd.Function):
         ops.count_fixup(ga, cnt, graph.by_dst, g_ab[:, :h])
         a, b = (ab[:, :h], ab[:, h:]) if ab is not None else (ga, ga)     # not read where the edge pass left bits
         g_we = ops._run_backward_src(a, b, ga, ea_t, w_edge, graph.by_src, graph, g_ab[:, h:], maskbits)
-        gx = nt(gz, wt_out[:f], g_ab, w_nodes.t().contiguous()) if ctx.needs_input_grad[0] else None
-        g_wn = gemm_tn8(g_ab, rx) if ctx.needs_input_grad[2] else None
-        return gx, None, g_wn, g_we if ctx.needs_input_grad[3] else None, g_wout if ctx.needs_input_grad[4] else None, None
+        gx = nt(gz, wt_out[:f], g_ab, w_nodes.t().contiguous()) if need_x else None
+        g_wn = gemm_tn8(g_ab, rx) if need_wn else None
+        return gx, None, g_wn, g_we if need_we else None, g_wout, None
 
 
 class _EgnnLayerFn(torch.autograd.Function):

@@ -62,3 +62,47 @@ def test_update_with_a_frozen_weight_takes_no_more_than_its_gradients(dtype):
     both = gemm_nn(torch.where(y > 0, gy, torch.zeros((), dtype=dtype, device="cuda")), w)
     for p, q in ((got, want), (got, (both[:, :f], both[:, f:]))):
         assert all(torch.equal(s, t) for s, t in zip(p, q))
+
+
+def large_graph(n, e):
+    gen = torch.Generator().manual_seed(7)
+    return torch.randint(0, n, (2, e), generator=gen).cuda(), torch.rand(e, 4, generator=gen).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,h,dtype", [(64, 64, torch.float32), (11, 50, torch.float32), (300, 64, torch.float32), (64, 64, torch.bfloat16)])
+def test_layer_with_frozen_weights_keeps_and_computes_what_is_wanted(f, h, dtype):
+    """Only the weight gradients read 8-bit rows: x's for either weight, aggr's for the update's.  What is wanted is what the
+    whole set of gradients has."""
+    from mpnn_amd import MPNNLayerSum
+    n = 3000
+    ei, ea = large_graph(n, 15000)
+    ea = ea.to(dtype)
+    torch.manual_seed(0)
+    layer = MPNNLayerSum(f, 4, h, checkpoint="int8").cuda().to(dtype)
+    x = torch.randn(n, f, device="cuda").relu().to(dtype)
+    gy = torch.randn(n, h, device="cuda").to(dtype)
+    names = [k for k, _ in layer.named_parameters()]
+
+    def grads(wanted, want_x):
+        for k, p in layer.named_parameters():
+            p.requires_grad_(k in wanted)
+        leaf = x.clone().requires_grad_(want_x)
+        held = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: held.append(t) or t, lambda t: t):
+            y = layer(leaf, ei, ea)
+        ins = ([leaf] if want_x else []) + [p for k, p in layer.named_parameters() if k in wanted]
+        out = torch.autograd.grad(y, ins, gy)
+        return dict(zip((["x"] if want_x else []) + [k for k in names if k in wanted], out)), sum(t.dtype == torch.int8 for t in held)
+
+    full, rows = grads(names, True)
+    assert rows == 2
+    tol = 2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -18     # the update's sums may run in another order without kept rows
+    for wanted, rows_wanted in ((["linear_out.weight"], 2), (["fused_linear.weight"], 1), (["linear_3.weight"], 0), ([], 0),
+                                (["fused_linear.weight", "linear_3.weight"], 1)):
+        got, rows = grads(wanted, True)
+        assert rows == rows_wanted, (wanted, rows)
+        for k, g in got.items():
+            assert float((g.double() - full[k].double()).norm()) <= tol * float(full[k].double().norm()), (wanted, k)
+    got, rows = grads(["fused_linear.weight"], False)
+    assert rows == 1 and float((got["fused_linear.weight"].double() - full["fused_linear.weight"].double()).norm()) <= tol * float(full["fused_linear.weight"].double().norm())
