@@ -603,7 +603,8 @@ int32_t mpnn_region_layer_bwd(const mpnn_island_layer* desc, int32_t max_nodes, 
  * norm(v) = v / sqrt(mean(v^2) + eps) (MPNN_NORM_RMS) or (v - mean) / sqrt(var(v) + eps) (MPNN_NORM_LAYER).
  * block, residual [N, H]; gate by gate_kind: none, [H], one value per row ([N] with stride ldg), or [N, H]; post_w,
  * post_b, w, b [H] or NULL (1 and 0); residual NULL counts as zeros.  All of one dtype; 1 <= H <= 2048.  Rows move
- * as 16-byte vectors when H, every address and every row stride allow it, column by column otherwise.
+ * four columns at a time (16 bytes in float32, 8 in bfloat16) where H, every address and every row stride allow it, column by
+ * column otherwise.
  *
  * mpnn_block_norm_fwd writes stream and / or normed (a NULL one is not computed).
  * mpnn_block_norm_bwd reads the forward's inputs again and g_stream, g_normed (NULL: zeros), and writes whichever of
@@ -643,10 +644,10 @@ int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
  *   from); G and Gout [N, M] of dtype, any row stride.
  * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * x_scale[n] * w_scale[m] + bias[m]); the sum is exact, the scales
  *   follow in float32 in the order that stays in its range (x_scale first where it is at most 1, else last).  x_dtype
- *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits first, in the workspace
- *   (mpnn_linear_int8_workspace_bytes, 16-byte aligned).  W [M, ldw] 8-bit rows with w_scale [M]; bias [M]
- *   of y_dtype or NULL.  8-bit rows 16-byte aligned, strides multiples of 16 and (mpnn_linear_int8) at most
- *   2^22; K <= 8192, M <= 2^20.
+ *   MPNN_I8: X holds 8-bit rows with scales x_scale; MPNN_F32 / MPNN_BF16: X [N, K] is taken to 8 bits on the way, in
+ *   registers or, where mpnn_linear_int8_workspace_bytes is not 0, in the workspace first (16-byte aligned).  W [M, ldw]
+ *   8-bit rows with w_scale [M]; bias [M] of y_dtype or NULL.  8-bit rows 16-byte aligned, strides multiples of 16 and
+ *   (mpnn_linear_int8) at most 2^22; K <= 8192, M <= 2^20.
  * mpnn_gemm_tn8         dW[M, K + K2] = sum_n (G * open)[n, :]^T [scale[n] Q[n, :] | scale2[n] Q2[n, :]]
  *   G, dW, Gout of dtype; bits (mpnn_relu_bits of the layer's output) or NULL select the entries of G that count; Gout
  *   (optional, [N, M]) receives G * open.  Q2, scale2: optional (K2 = 0).  8-bit rows 4-byte aligned; row strides at

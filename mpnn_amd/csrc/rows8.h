@@ -31,29 +31,6 @@ __device__ __forceinline__ uint32_t quant_word(float a, float b, float c, float 
   return (lo | hi) & q.keep;
 }
 
-// V consecutive outputs of a row; `left` of them exist.
-template <typename Y, int V>
-__device__ __forceinline__ void store_outputs(Y* p, const float (&v)[V], int left, bool wide) {
-  if (wide && left >= V) {
-    if constexpr (sizeof(Y) == 4) {
-#pragma unroll
-      for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-      uint32_t w[V / 2];
-#pragma unroll
-      for (int j = 0; j < V; j += 2) w[j / 2] = pack_bf16(v[j], v[j + 1]);
-      if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-      else
-#pragma unroll
-        for (int j = 0; j < V / 2; j += 4) *reinterpret_cast<uint4*>(p + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < left) p[j] = f32_to_scalar<Y>(v[j]);
-  }
-}
-
 // 16 bytes to a row that is not read here again.  Rows of whole 64-byte lines leave past the L2, which keeps the operands;
 // other rows share lines with their neighbours, and the L2 must put the parts together: 1 M x 100 float32 results from
 // 8-bit rows of 100 take 207 us past it and 147 through it, 1 M x 128 100 and 129.
@@ -82,7 +59,9 @@ struct Patch {
   static constexpr int VEC = 16 / sizeof(Y), CHUNKS = COLS / VEC, BYTES = ROWS * COLS * sizeof(Y);
   char* base;
   __device__ __forceinline__ void put(int row, int chunk, const float (&v)[VEC]) const {
-    store_outputs<Y, VEC>(reinterpret_cast<Y*>(base + row * (COLS * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16), v, VEC, true);
+    char* const p = base + row * (COLS * (int)sizeof(Y)) + ((chunk ^ row) & (CHUNKS - 1)) * 16;
+    if constexpr (sizeof(Y) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
   }
   // To rows r0 .. of y [N, ldy], outputs m .. m + COLS - 1 of which those below `end` exist, `width` bytes at a time (see
   // store_width).
