@@ -22,12 +22,15 @@ inline int32_t fail(int32_t code, const char* fmt, ...) {
   return code;
 }
 
+// (The runtime keeps a failed call's error until it is asked for: left there, the next launch's check would report it.)
 #define MPNN_HIP_CHECK(expr)                                                              \
   do {                                                                                    \
     hipError_t e_ = (expr);                                                               \
-    if (e_ != hipSuccess)                                                                 \
+    if (e_ != hipSuccess) {                                                               \
+      (void)hipGetLastError();                                                            \
       return ::mpnn::fail(MPNN_E_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), \
                           __FILE__, __LINE__);                                            \
+    }                                                                                     \
   } while (0)
 
 #define MPNN_LAUNCH_CHECK(name)                                                           \
