@@ -10,11 +10,12 @@
 //
 // Two kernels:
 //   rows    K <= 512, weights resident in LDS: x is read once as it lies, taken to 8 bits in registers and multiplied
-//           from there.  Bound by memory: 4 M rows of 128 -> 256 in 0.64 ms (bfloat16, 4.8 TB/s) and 1.19 ms (float32, 5.2
-//           TB/s; a copy reaches 4.9), Flickr's 89,250 of 500 -> 192 in 56 us (float32, 4.4 TB/s).
+//           from there.  Bound by memory: 4 M rows of 128 -> 256 in 0.60 to 0.67 ms (bfloat16, 4.6 to 5.1 TB/s) and 1.20 ms
+//           (float32, 5.1 TB/s; a copy reaches 4.9), Flickr's 89,250 of 500 -> 192 in 57 us (float32, 4.3 TB/s).
 //   tiles   both sides staged through LDS in steps of 128 bytes by asynchronous copies.  65,536 x 1024 -> 2048 to
-//           bfloat16 in 216 us (1270 TOP/s), 4096^3 in 80 us (1710 TOP/s).  What bounds it: operand reads from LDS (192
-//           KiB per step of 128 and CU, three quarters of the matrix cores' time) and, for short K, the results.
+//           bfloat16 in 178 us (1540 TOP/s), 4096^3 in 74 us (1860 TOP/s; a large library product reaches 1990).  What bounds
+//           it: operand reads from LDS (192 KiB per step of 128 and CU, three quarters of the matrix cores' time) and, for
+//           short K, the results.
 #include "common.h"
 #include "rows8.h"
 

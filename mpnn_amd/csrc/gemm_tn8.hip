@@ -17,8 +17,8 @@
 //   strips x tiles < 8: the waves left over share the rows of a slab; their sums meet in LDS at the end, in wave order.
 // One partial tile per block, added in block order by a second launch: no atomics, the same bits on every run.
 // Measured on 4 M rows: float32 256 x 128 0.97 ms = 4.8 TB/s, 128 x [128 | 128] with the relu's bits and g * open
-// written 1.13 ms = 4.6 TB/s; bfloat16 256 x 128 0.63 ms = 4.1 TB/s, 128 x [128 | 128] with both 0.90 ms = 3.5 TB/s (a
-// copy reaches 4.9).  What bounds bfloat16 there: the pieces are made once per matrix of q for half the bytes of g.
+// written 1.13 ms = 4.6 TB/s; bfloat16 256 x 128 0.65 ms = 4.0 TB/s, 128 x [128 | 128] with both 0.87 to 0.93 ms = 3.4 to
+// 3.6 TB/s (a copy reaches 4.9).  What bounds bfloat16 there: the pieces are made once per matrix of q for half the bytes of g.
 // Slabs of 64 rows instead of 128 for two column tiles took 1.13 ms, row clamps instead of whole slabs 20 % more.
 #include "common.h"
 #include "rowio.h"

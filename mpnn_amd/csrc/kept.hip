@@ -9,13 +9,13 @@
 // whole row segments.
 //
 //   bfloat16   a lane's 16-byte loads are the matrix operand: (row i, group g) holds columns 32 s + 8 g .. + 7 of step s.
-//              Bound by memory: 4 M rows, 128 + 128 -> 128, in 0.86 to 0.90 ms (4.5 to 4.7 TB/s; a copy reaches 4.9), where a
+//              Bound by memory: 4 M rows, 128 + 128 -> 128, in 0.90 to 0.96 ms (4.2 to 4.5 TB/s; a copy reaches 4.9), where a
 //              product, two quantising passes and a pass over y took 0.64 + 0.60 + 0.24 ms.
 //   float32    the three bfloat16 pieces and six products per pair of k_gemm_nt (gemm.hip) in its order, so that y is the same
 //              to the bit with and without kept rows.  The weights' pieces lie in LDS, cut once per block; weights that do
-//              not fit go in two slices, and x is read once per slice.  Bound by the matrix cores: 4 M rows, 128 -> 256, in 1.70 ms
-//              (0.92 PFLOP/s of piece products, where a large bfloat16 product reaches 1.28; the separate passes 2.29), 128 -> 128
-//              in 0.94 (1.44); 1 M rows, 64 + 64 -> 64, in 197 us (330).
+//              not fit go in two slices, and x is read once per slice.  Bound by the matrix cores: 4 M rows, 128 -> 256, in 1.79 ms
+//              (0.88 PFLOP/s of piece products, where a large bfloat16 product reaches 1.28; the separate passes 2.29), 128 -> 128
+//              in 0.95 (1.44); 1 M rows, 64 + 64 -> 64, in 195 us (330).
 //
 // Without kept rows the same kernels are the input gradient of those calls, y = x W for W as it lies [K, M]: brought into
 // place on its way to LDS, it saves the pass that transposes it (with that pass and gemm_nt: 18,432 x 64 -> 64 float32 16 us,

@@ -397,10 +397,14 @@ _ONES = {}
 
 
 def _ones(n: int, device) -> torch.Tensor:
-    """[n, 1] ones (the right-hand side that turns a weight-gradient product into column sums), kept per device."""
-    t = _ONES.get(device)
+    """[n, 1] ones (the right-hand side that turns a weight-gradient product into column sums), kept per device and stream.
+    A call that is captured gets its own: what a recorded graph fills holds nothing before its first replay."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.ones((n, 1), dtype=torch.float32, device=device)
+    key = (device, _lib.stream_handle(device))
+    t = _ONES.get(key)
     if t is None or t.size(0) < n:
-        t = _ONES[device] = torch.ones((max(n, 1024), 1), dtype=torch.float32, device=device)
+        t = _ONES[key] = torch.ones((max(n, 1024), 1), dtype=torch.float32, device=device)
     return t[:n]
 
 
