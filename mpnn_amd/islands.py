@@ -43,9 +43,9 @@ class Plan:
 
 def plan_for(graph: MPGraph, f: int, h: int, fe: int, egnn: bool) -> Plan | None:
     """The tile shape for this layer on this graph, or None when the island kernels do not apply (no islands known,
-    islands too large or too many, widths outside the kernels' range)."""
+    islands too large or too many, widths outside the kernels' range, no edge at all)."""
     isl = getattr(graph, "islands", None)
-    if isl is None:
+    if isl is None or graph.num_edges == 0:
         return None
     key = (f, h, fe, egnn, COUNT_MAX, REGIONS_ENABLED)
     plans = graph._scratch.setdefault("island_plans", {})    # per graph: the answer depends on the shapes only
