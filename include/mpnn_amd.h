@@ -639,7 +639,7 @@ int32_t mpnn_block_norm_bwd(const mpnn_block_norm* desc, mpnn_stream_t stream);
  *
  * mpnn_quantize_rows    X [N, K] (dtype, any row stride) -> Q [N, ldq] (16-byte aligned, ldq a multiple of 16; the
  *   bytes behind K are written as zeros), scale [N].  1 <= K <= 8192.
- * mpnn_relu_bits        bits [N][ceil(M / 32)] words: bit i of word w is set unless Y[n, 32 w + i] <= 0.
+ * mpnn_relu_bits        bits [N][ceil(M / 32)] words: bit i of word w is set unless Y[n, 32 w + i] <= 0.  M <= 2^30.
  * mpnn_open_entries     Gout[n, m] = G[n, m] where bit m of such bits is set, zero elsewhere (the gradient of the relu they came
  *   from); G and Gout [N, M] of dtype, any row stride.
  * mpnn_linear_int8      Y[n, m] = act((sum_k xq wq) * x_scale[n] * w_scale[m] + bias[m]); the sum is exact, the scales

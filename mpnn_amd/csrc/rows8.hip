@@ -18,6 +18,7 @@ namespace mpnn {
 namespace {
 
 constexpr int kRows8MaxK = 8192;
+constexpr int kBitsMaxM = 1 << 30;   // a row's columns and their padding count in 32 bits
 
 struct QuantArgs {
   const void* x;
@@ -215,7 +216,7 @@ int32_t mpnn_quantize_rows(const void* x, int64_t ldx, int32_t dtype, int64_t N,
 
 int32_t mpnn_relu_bits(const void* y, int64_t ldy, int32_t dtype, int64_t N, int32_t M, void* bits, mpnn_stream_t stream) {
   if (dtype != MPNN_F32 && dtype != MPNN_BF16) return fail(MPNN_E_INVALID, "mpnn_relu_bits: dtype %d", dtype);
-  if (N < 0 || M < 1 || ldy < M) return fail(MPNN_E_INVALID, "mpnn_relu_bits: N=%lld M=%d ldy=%lld", (long long)N, M, (long long)ldy);
+  if (N < 0 || M < 1 || M > kBitsMaxM || ldy < M) return fail(MPNN_E_INVALID, "mpnn_relu_bits: N=%lld M=%d ldy=%lld", (long long)N, M, (long long)ldy);
   if (N == 0) return MPNN_OK;
   if (!y || !bits) return fail(MPNN_E_INVALID, "mpnn_relu_bits: null pointer argument");
   const int pitch = (M + 31) / 32 * 4;
@@ -237,18 +238,18 @@ int32_t mpnn_relu_bits(const void* y, int64_t ldy, int32_t dtype, int64_t N, int
 int32_t mpnn_open_entries(const void* g, int64_t ldg, int32_t dtype, const void* bits, void* out, int64_t ldo, int64_t N, int32_t M,
                           mpnn_stream_t stream) {
   if (dtype != MPNN_F32 && dtype != MPNN_BF16) return fail(MPNN_E_INVALID, "mpnn_open_entries: dtype %d", dtype);
-  if (N < 0 || M < 1 || ldg < M || ldo < M)
+  if (N < 0 || M < 1 || M > kBitsMaxM || ldg < M || ldo < M)
     return fail(MPNN_E_INVALID, "mpnn_open_entries: N=%lld M=%d ldg=%lld ldo=%lld", (long long)N, M, (long long)ldg, (long long)ldo);
   if (N == 0) return MPNN_OK;
   if (!g || !bits || !out) return fail(MPNN_E_INVALID, "mpnn_open_entries: null pointer argument");
-  const int64_t pitch = ((int64_t)M + 31) / 32 * 4;
+  const int pitch = (M + 31) / 32 * 4;
   const int vec = dtype == MPNN_BF16 ? 8 : 4;
   const bool wide = M % 8 == 0 && (((uintptr_t)g | (uintptr_t)out) & 15) == 0 && ldg % vec == 0 && ldo % vec == 0;
-  int64_t blocks = (N * (((int64_t)M + 7) / 8) + kBlock - 1) / kBlock;
+  int64_t blocks = (N * ((M + 7) / 8) + kBlock - 1) / kBlock;
   if (blocks > 4 * kMaxBlocks) blocks = 4 * kMaxBlocks;
   auto launch = [&](auto kernel, auto t) {
     typedef decltype(t) T;
-    kernel<<<(int)blocks, kBlock, 0, stream>>>(static_cast<const T*>(g), ldg, N, M, static_cast<const uint8_t*>(bits), (int)pitch,
+    kernel<<<(int)blocks, kBlock, 0, stream>>>(static_cast<const T*>(g), ldg, N, M, static_cast<const uint8_t*>(bits), pitch,
                                                static_cast<T*>(out), ldo);
   };
   if (dtype == MPNN_BF16) wide ? launch(k_open_entries<bf16_t, true>, bf16_t()) : launch(k_open_entries<bf16_t, false>, bf16_t());

@@ -38,6 +38,10 @@ def test_open_entries_refuses_before_any_launch():
     for bad in (dict(dt=2), dict(n=-1), dict(m=0), dict(ldg=15), dict(ldo=15), dict(g=None), dict(bits=None), dict(out=None)):
         assert call(**bad) == -1, bad
     assert call(n=0) == 0
+    # rows whose columns 32 bits cannot count with their padding
+    wide = dict(m=(1 << 31) - 1, ldg=1 << 31, ldo=1 << 31)
+    assert call(**wide) == -1
+    assert lib.mpnn_relu_bits(p, 1 << 31, 0, 4, (1 << 31) - 1, p, None) == -1
 
 
 @pytest.mark.gpu
