@@ -191,8 +191,8 @@ class _LayerFn(torch.autograd.Function):
 class _KeptLayerFn(torch.autograd.Function):
     """The layer with its inputs held in 8 bits between the passes (rows8.py): x and aggr as 8-bit rows, the relu of the
     update in one bit per entry, the projection not at all where the edge pass left its own relu bits.  Per node of width
-    H in float32: 2 H + H / 8 bytes and the edge pass's counts and bits instead of 16 H bytes more.  Same calls as
-    _LayerFn's general path otherwise; the weight gradients take the values that the 8-bit rows stand for."""
+    H in float32: 2 H + H / 8 bytes where _LayerFn holds 20 H (x, the projection, aggr, the output); the edge pass's counts and
+    bits come on top of either.  Same calls as _LayerFn's general path otherwise; the weight gradients take the values that the 8-bit rows stand for."""
 
     @staticmethod
     def forward(ctx, x, edge_attr, w_nodes, w_edge, w_out, graph: MPGraph):

@@ -466,7 +466,8 @@ def partitioned_layer(layer, x_local: torch.Tensor, pg: PartitionedGraph, edge_a
     """One MPNN layer on the local destination range (same arithmetic as layer.forward on the whole graph).
 
     ``halo``: the exchange to use (default: a padded all-gather); build it once per PartitionedGraph and pass it to
-    every layer.  ``x_all``: the layer's input for ALL nodes, replicated on every rank (a first layer reading the
+    every layer.  A layer's ``checkpoint`` option has no effect here: what waits for the backward stays in its type.
+    ``x_all``: the layer's input for ALL nodes, replicated on every rank (a first layer reading the
     dataset's features): no exchange, and no gradient with respect to the input.
     ``aggregate_fn`` / ``dense_fns`` = (project, update) replace the HIP operators by stand-ins with the same
     signatures; they exist for the CPU rehearsals of the exchange logic (the kernels need a GPU)."""

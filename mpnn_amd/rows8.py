@@ -45,7 +45,7 @@ class Rows8:
         return self.values.stride(0) if self.values.size(0) > 1 else _pitch(self.values.size(1))
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The values the rows stand for, rounded once to ``dtype``."""
+        """The values the rows stand for: a whole number times the scale in float32, rounded once, then to ``dtype``."""
         return (self.values.float() * self.scale.unsqueeze(1)).to(dtype)
 
 
